@@ -29,12 +29,14 @@ DEV_TABLE_FULL = 0x4
 DEV_OOM = 0x8
 DEV_TIMEOUT = 0x10
 DEV_CTX_RANGE = 0x20
+DEV_BAD_PLAN = 0x40
 
 PARTITION_BALANCED = -1  # CLOVER_B200_PARTITION_BALANCED: the balanced split
 
-F32, F16, BF16, FP8_E4M3 = 0, 1, 2, 3
+F32, F16, BF16, FP8_E4M3, INT8 = 0, 1, 2, 3, 4
 _DTYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,
-          torch.float8_e4m3fn: FP8_E4M3}  # fp8: KV caches only
+          torch.float8_e4m3fn: FP8_E4M3, torch.int8: INT8}  # fp8, int8: KV caches only
+_SCALED = (torch.int8, torch.float8_e4m3fn)  # caches that may carry scales
 
 # Every symbol include/clover_b200.h declares: name -> (restype, argtypes)
 _P = ctypes.c_void_p
@@ -77,6 +79,18 @@ SIGNATURES = {
     "clover_b200_paged_decode_noalloc": (ctypes.c_int, [
         _P, _I64, _P, _I64, _I32, _P, _P, _I32, _I64, _I32, _P, _I32, _P, _P, _P,
         _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _I32, _P, _P]),
+    "clover_b200_plan_step": (ctypes.c_int, [
+        _P, _P, _I32, _P, _I32, _P, _P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _I32, _P, _P]),
+    "clover_b200_kv_append_scaled": (ctypes.c_int, [
+        _P, _P, _P, _P, _I32, _I64, _I64, _P, _P, _I32, _I64, _I64, _P, _I64, _I32, _I32, _I32, _I32,
+        _I64, _P, _P]),
+    "clover_b200_attend_workspace_bytes": (ctypes.c_int64, [_I32] * 11),
+    "clover_b200_scaled_decode": (ctypes.c_int, [
+        _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _I32, _I64, _I32, _P, _P, _I64, _I32, _P, _I32, _P, _P,
+        _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _P, _I64, _P, _P]),
+    "clover_b200_diff_decode": (ctypes.c_int, [
+        _P, _I64, _P, _I64, _I32, _P, _P, _P, _P, _I32, _I64, _I32, _P, _P, _I64, _I32, _P, _I32, _P, _P,
+        _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F, _P, _P, _F, _F, _P, _I64, _P, _P]),
 }
 NOALLOC_SCRATCH_BYTES = 16 << 20  # CLOVER_B200_NOALLOC_SCRATCH_BYTES
 
@@ -311,6 +325,232 @@ def decode_step(out, q, k_cache, v_cache, k_new, v_new, block_tables, query_star
         float(score_scale), partition_tokens, _ptr(workspace), ws_bytes, _ptr(status),
         _stream(q.device))
     _check(rc, "clover_b200_decode_step")
+
+
+# ---------------------------------------------------------------- step plan, 8-bit caches, differential decode
+def _one_device(what, *ts) -> torch.device:
+    """The device all given tensors live on (None is skipped)."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and (t.device != dev or not t.is_cuda):
+            raise ValueError(f"{what}: tensors must be on one CUDA device, got {t.device} beside {dev}")
+    return dev
+
+
+def _call_on(dev: torch.device, fn, *args) -> int:
+    """Call a launching entry point with its tensors' device current and its
+    current stream as the last argument."""
+    if dev.index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    with torch.cuda.device(dev):
+        return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _index_i32(what, *ts) -> None:
+    for t in ts:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise TypeError(f"{what}: index tensors must be contiguous int32")
+
+
+def plan_step(free_stack, free_top, tables, table_len, seq_lens, rows, n_new, block_size,
+              query_start_loc, ctx_lens, slot_mapping, status):
+    """Plan one step on the GPU (``clover_b200_plan_step``): grow the tables of
+    ``rows`` for ``n_new`` tokens each, fill ``query_start_loc [n + 1]`` and, for up to
+    ``slot_mapping.numel()`` tokens, ``ctx_lens`` and ``slot_mapping``, and advance
+    ``seq_lens``, ``table_len`` and ``free_top``.  No host sync; a step that does not
+    fit changes nothing and sets ``status``."""
+    dev = _one_device("plan_step", free_stack, free_top, tables, table_len, seq_lens, rows, n_new,
+                      query_start_loc, ctx_lens, slot_mapping, status)
+    _index_i32("plan_step", free_stack, free_top, tables, table_len, seq_lens, rows, n_new,
+               query_start_loc, ctx_lens, status)
+    if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous():
+        raise TypeError("plan_step: slot_mapping must be contiguous int64")
+    n, m = rows.numel(), slot_mapping.numel()
+    if n_new.numel() != n or query_start_loc.numel() != n + 1 or ctx_lens.numel() != m:
+        raise ValueError(f"plan_step: {n} rows need {n} counts and {n + 1} offsets, "
+                         f"{m} slots need {m} contexts")
+    if (tables.dim() != 2 or table_len.numel() != tables.shape[0] or seq_lens.numel() != tables.shape[0]
+            or free_top.numel() != 1):
+        raise ValueError("plan_step: tables [rows, width], table_len [rows], seq_lens [rows], free_top [1]")
+    rc = _call_on(dev, lib().clover_b200_plan_step, free_stack.data_ptr(), free_top.data_ptr(),
+                  free_stack.numel(), tables.data_ptr(), tables.shape[1], table_len.data_ptr(),
+                  seq_lens.data_ptr(), tables.shape[0], rows.data_ptr(), n_new.data_ptr(), n, block_size,
+                  query_start_loc.data_ptr(), ctx_lens.data_ptr(), slot_mapping.data_ptr(), m,
+                  _ptr(status))
+    if rc != OK:
+        _check(rc, "clover_b200_plan_step")
+
+
+def _check_scaled_cache(what, k_cache, v_cache, k_scales, v_scales):
+    """Shape rules of an 8-bit cache [.., num_blocks, bs, H, D] and its scales
+    [.., num_blocks, H, bs] (one layer, or several in front)."""
+    if k_cache.dtype not in _SCALED or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"{what}: the cache must be int8 or float8_e4m3fn, got {k_cache.dtype}")
+    if k_scales is None or v_scales is None:
+        raise ValueError(f"{what}: an 8-bit cache needs k_scales and v_scales")
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+        raise TypeError(f"{what}: scales must be float32")
+    nb, bs, h, _ = k_cache.shape[-4:]
+    want = k_cache.shape[:-4] + (nb, h, bs)
+    if v_cache.shape != k_cache.shape or k_scales.shape != want or v_scales.shape != want:
+        raise ValueError(f"{what}: scales {tuple(k_scales.shape)} do not fit a cache "
+                         f"{tuple(k_cache.shape)} (expected {tuple(want)})")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous()
+            and v_scales.is_contiguous()):
+        raise ValueError(f"{what}: caches and scales must be contiguous")
+
+
+def kv_append_scaled(k_cache, v_cache, k_scales, v_scales, k_new, v_new, slot_mapping, status):
+    """Quantise new tokens' K/V into an 8-bit cache with scales
+    (``clover_b200_kv_append_scaled``): caches [num_blocks, bs, H, D] int8 or
+    float8_e4m3fn, scales [num_blocks, H, bs] float32, k_new/v_new [n, H, D] f32,
+    f16 or bf16 (token stride free); or every one with a layer axis in front."""
+    what = "kv_append_scaled"
+    dev = _one_device(what, k_cache, v_cache, k_scales, v_scales, k_new, v_new, slot_mapping, status)
+    many = k_cache.dim() == 5
+    if k_cache.dim() not in (4, 5) or k_new.dim() != k_cache.dim() - 1 or v_new.shape != k_new.shape:
+        raise ValueError(f"{what}: cache {tuple(k_cache.shape)} and new K/V {tuple(k_new.shape)} do not fit")
+    _check_scaled_cache(what, k_cache, v_cache, k_scales, v_scales)
+    nb, bs, h, d = k_cache.shape[-4:]
+    layers = k_cache.shape[0] if many else 1
+    n = k_new.shape[-3]
+    if tuple(k_new.shape) != ((layers,) if many else ()) + (n, h, d):
+        raise ValueError(f"{what}: new K/V {tuple(k_new.shape)} do not fit a cache {tuple(k_cache.shape)}")
+    if k_new.dtype not in (torch.float32, torch.float16, torch.bfloat16) or v_new.dtype != k_new.dtype:
+        raise TypeError(f"{what}: new K/V must be float32, float16 or bfloat16")
+    if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or slot_mapping.numel() != n:
+        raise ValueError(f"{what}: slot_mapping must be {n} contiguous int64 values")
+    if n == 0:
+        return
+    if (k_new.stride(-1) != 1 and d > 1) or (k_new.stride(-2) != d and h > 1) or v_new.stride() != k_new.stride():
+        raise ValueError(f"{what}: each token's [H, D] row must be contiguous")
+    rc = _call_on(dev, lib().clover_b200_kv_append_scaled, k_cache.data_ptr(), v_cache.data_ptr(),
+                  k_scales.data_ptr(), v_scales.data_ptr(), _DTYPE[k_cache.dtype],
+                  k_cache.stride(0) if many else 0, k_scales.stride(0) if many else 0,
+                  k_new.data_ptr(), v_new.data_ptr(), _DTYPE[k_new.dtype],
+                  k_new.stride(0) if many else 0, k_new.stride(-3) if n > 1 else h * d,
+                  slot_mapping.data_ptr(), n, layers, h, d, bs, nb, _ptr(status))
+    if rc != OK:
+        _check(rc, "clover_b200_kv_append_scaled")
+
+
+def attend_workspace_bytes(n_seqs, n_rows, max_queries_per_seq, max_ctx_len, num_q_heads, num_kv_heads,
+                           head_dim, block_size, kv_dtype, q_dtype, differential=False) -> int:
+    """Workspace of scaled_decode (or diff_decode) on the current device."""
+    nb = int(lib().clover_b200_attend_workspace_bytes(
+        n_seqs, n_rows, max_queries_per_seq, max_ctx_len, num_q_heads, num_kv_heads, head_dim,
+        block_size, dtype_code(kv_dtype), dtype_code(q_dtype), int(differential)))
+    if nb < 0:
+        raise CloverB200Error(lib().clover_b200_last_error().decode(errors="replace"))
+    return nb
+
+
+_attend_ws = {}  # workspace bytes by (device, sizes): a query per new shape, not per call
+
+
+def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables, query_start_loc,
+            ctx_lens, max_queries_per_seq, max_ctx_len, score_scale, k_new, v_new, seq_rows, workspace,
+            status, lam=None, norm_weight=None, eps=0.0, out_scale=1.0):
+    """Checks and call shared by scaled_decode and diff_decode."""
+    diff = lam is not None
+    dev = _one_device(what, q, out, k_cache, v_cache, k_scales, v_scales, block_tables, query_start_loc,
+                      ctx_lens, k_new, v_new, seq_rows, workspace, status, lam, norm_weight)
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"{what}: q [rows, Hq, D] and caches [num_blocks, bs, Hkv, D]")
+    nb, bs, hkv, d = k_cache.shape
+    rows, hq, dq = q.shape
+    if dq != d or out.shape != q.shape:
+        raise ValueError(f"{what}: q/out shape mismatch")
+    if q.stride(2) != 1 or q.stride(1) != d or out.stride(2) != 1 or out.stride(1) != d:
+        raise ValueError(f"{what}: each row's [Hq, D] must be contiguous")
+    if out.dtype != q.dtype or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"{what}: out dtype must equal q dtype, V's cache K's")
+    if k_scales is not None or not diff or k_cache.dtype in _SCALED:
+        _check_scaled_cache(what, k_cache, v_cache, k_scales, v_scales)
+    elif v_scales is not None or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{what}: caches must be contiguous; only an 8-bit cache has scales")
+    _index_i32(what, query_start_loc, ctx_lens, seq_rows, status)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1:
+        raise TypeError(f"{what}: block_tables must be int32 rows")
+    n_seqs = query_start_loc.numel() - 1
+    if ctx_lens.numel() < rows or n_seqs < 0:
+        raise ValueError(f"{what}: {rows} rows need {rows} contexts")
+    if (block_tables.shape[0] if seq_rows is None else seq_rows.numel()) < n_seqs:
+        raise ValueError(f"{what}: {n_seqs} sequences need as many table rows")
+    if (k_new is None) != (v_new is None):
+        raise ValueError(f"{what}: new K without new V")
+    if k_new is not None:
+        if k_new.shape != (rows, hkv, d) or v_new.shape != k_new.shape:
+            raise ValueError(f"{what}: new K/V must be [{rows}, {hkv}, {d}]")
+        if v_new.dtype != k_new.dtype or (k_scales is None and k_new.dtype != k_cache.dtype):
+            raise TypeError(f"{what}: new K/V dtype must match the cache")
+        if rows and (k_new.stride(2) != 1 or k_new.stride(1) != d or v_new.stride() != k_new.stride()):
+            raise ValueError(f"{what}: each token's [Hkv, D] row must be contiguous")
+    if diff:
+        if lam.dtype != torch.float32 or lam.shape != (hq,) or not lam.is_contiguous():
+            raise ValueError(f"{what}: lam must be {hq} contiguous float32 values")
+        if norm_weight is not None and (norm_weight.dtype != torch.float32 or norm_weight.shape != (d,)
+                                        or not norm_weight.is_contiguous()):
+            raise ValueError(f"{what}: norm_weight must be {d} contiguous float32 values")
+    if rows == 0 or n_seqs == 0:
+        return
+    if workspace is None:
+        key = (dev.index, n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d, bs, k_cache.dtype,
+               q.dtype, diff)
+        need = _attend_ws.get(key)
+        if need is None:
+            with torch.cuda.device(dev):
+                need = attend_workspace_bytes(*key[1:])
+            if len(_attend_ws) > 4096:
+                _attend_ws.clear()
+            _attend_ws[key] = need
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    args = (out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), dtype_code(q.dtype),
+            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+            dtype_code(k_cache.dtype), nb, bs, _ptr(k_new), _ptr(v_new),
+            0 if k_new is None else k_new.stride(0), 0 if k_new is None else dtype_code(k_new.dtype),
+            block_tables.data_ptr(), block_tables.stride(0), _ptr(seq_rows), query_start_loc.data_ptr(),
+            ctx_lens.data_ptr(), n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d,
+            float(score_scale))
+    tail = (_ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+            _ptr(status))
+    if diff:
+        rc = _call_on(dev, fn, *args, lam.data_ptr(), _ptr(norm_weight), float(eps), float(out_scale), *tail)
+    else:
+        rc = _call_on(dev, fn, *args, *tail)
+    if rc != OK:
+        _check(rc, "clover_b200_" + what)
+
+
+def scaled_decode(out, q, k_cache, v_cache, k_scales, v_scales, block_tables, query_start_loc, ctx_lens, *,
+                  max_queries_per_seq, max_ctx_len, score_scale, k_new=None, v_new=None, seq_rows=None,
+                  workspace=None, status=None):
+    """Paged decode over an 8-bit cache with scales (``clover_b200_scaled_decode``):
+    q/out [rows, Hq, D] f32, f16 or bf16 (row stride free), caches
+    [num_blocks, bs, Hkv, D] int8 or float8_e4m3fn, scales [num_blocks, Hkv, bs]
+    float32.  With k_new/v_new [rows, Hkv, D] every row's token is quantised into
+    position ctx - 1 first.  Rows past ``query_start_loc[-1]`` are left as they were.
+    ``workspace`` (attend_workspace_bytes) is allocated here by default."""
+    _attend("scaled_decode", lib().clover_b200_scaled_decode, out, q, k_cache, v_cache, k_scales, v_scales,
+            block_tables, query_start_loc, ctx_lens, max_queries_per_seq, max_ctx_len, score_scale, k_new,
+            v_new, seq_rows, workspace, status)
+
+
+def diff_decode(out, q, k_cache, v_cache, lam, block_tables, query_start_loc, ctx_lens, *,
+                max_queries_per_seq, max_ctx_len, score_scale, norm_weight=None, eps=1e-5, out_scale=1.0,
+                k_scales=None, v_scales=None, k_new=None, v_new=None, seq_rows=None, workspace=None,
+                status=None):
+    """Differential decode attention (``clover_b200_diff_decode``): the halves of
+    head_dim of q and K are two maps, out = softmax_1 V - lam[head] * softmax_2 V, then
+    (with ``norm_weight``) its RMS norm over head_dim times ``out_scale``.  Caches as
+    in :func:`paged_decode` (f32, f16, bf16) or 8-bit with scales; the rest as
+    :func:`scaled_decode`."""
+    if lam is None:
+        raise ValueError("diff_decode: lam is required")
+    _attend("diff_decode", lib().clover_b200_diff_decode, out, q, k_cache, v_cache, k_scales, v_scales,
+            block_tables, query_start_loc, ctx_lens, max_queries_per_seq, max_ctx_len, score_scale, k_new,
+            v_new, seq_rows, workspace, status, lam, norm_weight, eps, out_scale)
 
 
 # ---------------------------------------------------------------- peer memory / fused gather

@@ -59,6 +59,8 @@ extern "C" {
 #define CLOVER_B200_DEV_OOM           0x8  /* free stack exhausted (batch left unchanged) */
 #define CLOVER_B200_DEV_TIMEOUT      0x10  /* a bounded wait gave up                */
 #define CLOVER_B200_DEV_CTX_RANGE    0x20  /* a context exceeds max_ctx_len        */
+#define CLOVER_B200_DEV_BAD_PLAN     0x40  /* plan_step: a row out of range or twice, a
+                                              negative count, too many tokens (nothing changed) */
 
 /* ---- dtypes --------------------------------------------------------------- */
 #define CLOVER_B200_F32  0
@@ -69,6 +71,8 @@ extern "C" {
  * the decode takes it on the tensor-core path (head_dim 128 or 256, block
  * 16 or 32).  No counterpart in the reference, which keeps fp16/fp32 caches. */
 #define CLOVER_B200_FP8_E4M3 3
+/* KV cache with scales only (clover_b200_kv_append_scaled and its decodes). */
+#define CLOVER_B200_INT8 4
 
 /* Library version (major*10000 + minor*100 + patch). */
 CLOVER_B200_API int clover_b200_version(void);
@@ -390,6 +394,120 @@ CLOVER_B200_API int clover_b200_paged_decode_noalloc(void* out, int64_t out_row_
                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                              float score_scale, int32_t partition_tokens,
                              int32_t* dev_status, void* stream);
+
+/*
+ * Step plan on the GPU: from request lengths that live on the device to
+ * everything a step's append and decode take, in one launch and without the
+ * host.  Item i is table row rows[i] (negative: padding, no tokens) with
+ * n_new[i] >= 0 new tokens after the seq_lens[rows[i]] it holds.  The rows'
+ * tables grow to hold them, popping blocks as clover_b200_block_reserve does
+ * (item order, then table order); then
+ *   query_start_loc[n_items + 1]  exclusive sum of n_new
+ *   ctx_lens[max_tokens]          token j of item i: len_i + j + 1 (0 past the last token)
+ *   slot_mapping[max_tokens]      its flat cache slot (-1 past the last token)
+ * and seq_lens, table_len and *free_top are advanced, so a captured plan +
+ * append + decode can be replayed step after step.  seq_lens, table_len and
+ * the tables have num_rows rows.  All or nothing: if the blocks, a table row
+ * or max_tokens do not hold the step, or a row is out of range or stands in
+ * the batch twice, the status word gets OOM, TABLE_FULL or BAD_PLAN, no state
+ * changes and the layout is empty (zeros and -1).  At most 8192 items and
+ * 262144 rows.  Calls on one allocator state must be ordered by the caller.
+ * Replaces: append_slot for every request of a step (memory_manager.py:95-121)
+ * with get_kernel_inputs (:145-173).
+ */
+CLOVER_B200_API int clover_b200_plan_step(int32_t* free_stack, int32_t* free_top, int32_t num_blocks,
+                          int32_t* block_tables, int32_t table_stride, int32_t* table_len,
+                          int32_t* seq_lens, int32_t num_rows, const int32_t* rows,
+                          const int32_t* n_new, int32_t n_items, int32_t block_size,
+                          int32_t* query_start_loc, int32_t* ctx_lens, int64_t* slot_mapping,
+                          int32_t max_tokens, int32_t* dev_status, void* stream);
+
+/*
+ * KV append into an 8-bit cache with scales: token j's K and V rows (f32, f16
+ * or bf16, one per KV head) are stored in slot slot_mapping[j] as codes and
+ * one fp32 scale per (token, KV head), x ~ scale * code:
+ *   a = max |x|, scale = a / top, code = round(x * (top * (1 / a))), top = 127
+ *   (CLOVER_B200_INT8, to nearest even, within +-127) or 448
+ *   (CLOVER_B200_FP8_E4M3, the e4m3 value nearest, ties to even).
+ * a < 2^-100: zeros with scale 0.  A row with an infinity or NaN: scale NaN
+ * (attending to it gives NaN).  Caches as in clover_b200_kv_append with 1-byte
+ * elements; k_scales / v_scales are [num_blocks, num_kv_heads, block_size].
+ * n_layers > 1: the layers lie cache_layer_stride, scale_layer_stride and
+ * new_layer_stride elements apart (ignored for one layer).  Negative slots are
+ * skipped, slots past the cache raise BAD_SLOT; a slot must not stand in the
+ * mapping twice.  Any head_dim and alignment.
+ * Replaces: as clover_b200_kv_append; upstream caches hold fp16/fp32 only.
+ */
+CLOVER_B200_API int clover_b200_kv_append_scaled(void* k_cache, void* v_cache, float* k_scales, float* v_scales,
+                          int32_t kv_dtype, int64_t cache_layer_stride, int64_t scale_layer_stride,
+                          const void* k_new, const void* v_new, int32_t new_dtype,
+                          int64_t new_layer_stride, int64_t new_token_stride,
+                          const int64_t* slot_mapping, int64_t n_tokens, int32_t n_layers,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                          int64_t num_blocks, int32_t* dev_status, void* stream);
+
+/*
+ * Bytes of workspace clover_b200_scaled_decode (differential = 0) or
+ * clover_b200_diff_decode (1) needs for a call of these sizes; 0 for short
+ * contexts, -1 on invalid sizes.  It does not grow with the batch.
+ */
+CLOVER_B200_API int64_t clover_b200_attend_workspace_bytes(int32_t n_seqs, int32_t n_query_rows,
+                          int32_t max_queries_per_seq, int32_t max_ctx_len, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                          int32_t kv_dtype, int32_t q_dtype, int32_t differential);
+
+/*
+ * Paged decode over an 8-bit cache with scales (clover_b200_kv_append_scaled):
+ * as clover_b200_paged_decode with K row t = k_scales * codes, V row t =
+ * v_scales * codes; queries and outputs f32, f16 or bf16.  k_new / v_new (may
+ * be NULL; new_dtype f32, f16 or bf16): every query row's new token is
+ * quantised into position ctx_lens[r] - 1 first, as in
+ * clover_b200_decode_step.  Within a sequence ctx_lens must not decrease.  Rows
+ * at and past query_start_loc[n_seqs] are not touched; a masked token adds
+ * nothing, whatever it holds.  head_dim up to 256, any block_size; head_dim
+ * 64/128/256 with a block_size that is a multiple of 16 takes the tensor-core
+ * kernel (cache 16-byte aligned).  Workspace: clover_b200_attend_workspace_bytes,
+ * 16-byte aligned, not shared by calls that may overlap.
+ * Replaces: as clover_b200_paged_decode / clover_b200_decode_step.
+ */
+CLOVER_B200_API int clover_b200_scaled_decode(void* out, int64_t out_row_stride,
+                          const void* q, int64_t q_row_stride, int32_t q_dtype,
+                          void* k_cache, void* v_cache, float* k_scales, float* v_scales,
+                          int32_t kv_dtype, int64_t num_blocks, int32_t block_size,
+                          const void* k_new, const void* v_new, int64_t new_token_stride,
+                          int32_t new_dtype, const int32_t* block_tables, int32_t table_stride,
+                          const int32_t* seq_rows, const int32_t* query_start_loc,
+                          const int32_t* ctx_lens, int32_t n_seqs, int32_t n_query_rows,
+                          int32_t max_queries_per_seq, int32_t max_ctx_len, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, float score_scale,
+                          void* workspace, int64_t workspace_bytes, int32_t* dev_status,
+                          void* stream);
+
+/*
+ * Differential decode attention over the same paged caches.  The first half of
+ * a head's query and key dims is map 1, the second half map 2, values are
+ * whole:  o_m = softmax(score_scale * q_m . K_m^T) . V,
+ *   o = o_1 - lambda[head] * o_2          (lambda: [num_q_heads] fp32, device)
+ * and, with norm_weight ([head_dim] fp32, device; may be NULL),
+ *   out = o * rsqrt(mean(o^2) + eps) * norm_weight * out_scale.
+ * (out_scale only applies with the norm.)  head_dim is even.  Caches: f32, f16
+ * or bf16 (k_scales = v_scales = NULL; queries fp32 or of the cache's type,
+ * k_new / v_new of the cache's type), or 8-bit with scales.  Everything else
+ * as clover_b200_scaled_decode.  No counterpart in the reference.
+ */
+CLOVER_B200_API int clover_b200_diff_decode(void* out, int64_t out_row_stride,
+                          const void* q, int64_t q_row_stride, int32_t q_dtype,
+                          void* k_cache, void* v_cache, float* k_scales, float* v_scales,
+                          int32_t kv_dtype, int64_t num_blocks, int32_t block_size,
+                          const void* k_new, const void* v_new, int64_t new_token_stride,
+                          int32_t new_dtype, const int32_t* block_tables, int32_t table_stride,
+                          const int32_t* seq_rows, const int32_t* query_start_loc,
+                          const int32_t* ctx_lens, int32_t n_seqs, int32_t n_query_rows,
+                          int32_t max_queries_per_seq, int32_t max_ctx_len, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, float score_scale,
+                          const float* lambda, const float* norm_weight, float eps,
+                          float out_scale, void* workspace, int64_t workspace_bytes,
+                          int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus
 }
