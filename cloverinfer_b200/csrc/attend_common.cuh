@@ -65,6 +65,7 @@ struct AttendArgs {
   const float* lam;
   const float* norm_w;
   float eps, out_scale;
+  int32_t p_lo;  // softmax weights as two 16-bit terms (else one)
   // fused append (tensor-core path): row r's new K/V at position ctx[r] - 1
   const void* k_new;
   const void* v_new;
@@ -149,7 +150,7 @@ __device__ __forceinline__ void attend_check_seq(const AttendArgs& a, const SeqI
     raise_status(a.status, CLOVER_B200_DEV_CTX_RANGE);
 }
 
-// A worker's position: unit jj of segment h (of hc) of sequence b; seg0 is the
+// A worker's position: unit jj of segment h (of s.hc) of sequence b; seg0 is the
 // flat number of the segment's first unit.  Split launches end after `left`
 // units, whole launches at the last segment.
 struct Cursor {
@@ -165,8 +166,24 @@ struct Cursor {
     seg0 = base + h * s.n;
     left = units;
   }
+  // Whole launches: the first segment with units among sg, sg + workers, ...
+  __device__ __forceinline__ bool seek(const AttendArgs& a, int64_t sg) {
+    const int hcmax = a.hkv * a.chunks;
+    for (; sg < (int64_t)a.n_seqs * hcmax; sg += a.workers) {
+      b = (int)sg / hcmax;
+      h = (int)sg - b * hcmax;
+      s = seq_info(a, b);
+      if (h < s.hc && s.n > 0) {
+        jj = 0;
+        seg0 = (int)sg;
+        return true;
+      }
+    }
+    return false;
+  }
   // Next unit; false at the end.
   __device__ __forceinline__ bool next(const AttendArgs& a) {
+    if (a.whole) return ++jj < s.n || seek(a, (int64_t)seg0 + a.workers);
     if (--left <= 0) return false;
     if (++jj < s.n) return true;
     jj = 0;

@@ -43,7 +43,7 @@ attend_generic_kernel(const AttendArgs a) {
   pdl_wait();
   int per = 0, total = 0;
   Cursor cur;
-  int seg = 0;  // whole launches: the worker's segment
+  int seg = 0;  // whole launches: the worker's segment (empty ones too: their zeros)
   const int hcmax = a.hkv * a.chunks;
   if (!a.whole) {
     per = attend_plan(a, plan, total);
@@ -574,8 +574,9 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
               : new_dtype != kv_dtype)
       return set_error(CLOVER_B200_ERR_UNSUPPORTED, "%s: new K/V dtype %d", what, new_dtype);
   }
-  if (sh.mma && ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15))
-    return set_error(CLOVER_B200_ERR_INVALID_ARG, "%s: cache not 16-byte aligned", what);
+  if (sh.mma && ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+                  reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) & 15))
+    return set_error(CLOVER_B200_ERR_INVALID_ARG, "%s: cache or scales not 16-byte aligned", what);
   if (num_blocks * (int64_t)block_size > INT32_MAX)
     return set_error(CLOVER_B200_ERR_UNSUPPORTED, "%s: cache exceeds 2^31 slots", what);
   if (sh.bytes > 0 && (workspace == nullptr || workspace_bytes < sh.bytes ||
@@ -623,6 +624,8 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   a.norm_w = norm_weight;
   a.eps = eps;
   a.out_scale = out_scale;
+  // one fp16 weight term (2^-12) under a bf16 output, unless maps cancel
+  a.p_lo = 1;
   a.status = dev_status;
   a.wait_ns = wait_limit_ns();
   cudaStream_t s = (cudaStream_t)stream;
