@@ -2,9 +2,9 @@
 // one softmax map per head or two (differential attention): arguments, the
 // split of a step's work over its workers, and how a worker's result leaves it.
 //
-// Work: a unit is kUnitTok consecutive tokens of one segment; a segment is
-// (sequence b, KV head, column chunk) and holds n = ceil(ctx_b / kUnitTok)
-// units, ctx_b the context of the sequence's last row (rows are in causal
+// Work: a unit is 16 or 32 consecutive tokens (the kernel's choice) of one
+// segment; a segment is (sequence b, KV head, column chunk) and holds
+// n = ceil(ctx_b / unit) units, ctx_b the context of the sequence's last row (rows are in causal
 // order).  A column is one (query row, query head of the KV head's group,
 // map), so a KV tile is read once for all heads of a group, all new tokens and
 // both maps.  A worker is one warp.
@@ -27,10 +27,10 @@
 
 namespace clover {
 
-constexpr int kUnitTok = 16;
+constexpr int kUnitTok = 16;     // a unit is a multiple of this
 constexpr int kAttendWarps = 4;  // workers of a CTA
 constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kAttendMinUnits = 8;  // a worker's least range (128 tokens)
+constexpr int kAttendMinTok = 128;  // a worker's least range
 constexpr int kAttendMaxPerSm = 16; // workers per SM the workspace allows for
 
 struct AttendArgs {
@@ -49,6 +49,7 @@ struct AttendArgs {
   const int32_t* qsl;
   const int32_t* ctx;
   int32_t n_seqs, n_rows, max_ctx;
+  int32_t unit_log2;  // log2 of a unit's tokens
   int32_t hq, hkv, group, maps;  // maps: 1, or 2 for differential attention
   int32_t D, bs;
   int64_t num_blocks;
@@ -65,7 +66,6 @@ struct AttendArgs {
   const float* lam;
   const float* norm_w;
   float eps, out_scale;
-  int32_t p_lo;  // softmax weights as two 16-bit terms (else one)
   // fused append (tensor-core path): row r's new K/V at position ctx[r] - 1
   const void* k_new;
   const void* v_new;
@@ -122,7 +122,7 @@ __device__ __forceinline__ float attend_inv(float l, int lim) {
 // ------------------------------------------------------------------ cursor
 // One sequence of the batch as the cursor sees it.
 struct SeqInfo {
-  int row0, nq, n, hc;  // first row, rows, units per segment, segments
+  int row0, nq, ctx, n, hc;  // first row, rows, longest context, units per segment, segments
 };
 
 __device__ __forceinline__ SeqInfo seq_info(const AttendArgs& a, int b) {
@@ -131,13 +131,13 @@ __device__ __forceinline__ SeqInfo seq_info(const AttendArgs& a, int b) {
   s.nq = min(__ldg(a.qsl + b + 1), a.n_rows) - s.row0;
   s.n = 0;
   s.hc = 0;
+  s.ctx = 0;
   if (s.nq <= 0 || s.row0 < 0) {
     s.nq = 0;
     return s;
   }
-  int c = __ldg(a.ctx + s.row0 + s.nq - 1);
-  c = c < a.max_ctx ? c : a.max_ctx;
-  s.n = c > 0 ? (c + kUnitTok - 1) / kUnitTok : 0;
+  s.ctx = max(0, min(__ldg(a.ctx + s.row0 + s.nq - 1), a.max_ctx));
+  s.n = (s.ctx + (1 << a.unit_log2) - 1) >> a.unit_log2;
   const int ch = (s.nq * a.group * a.maps + a.cols - 1) / a.cols;
   s.hc = a.hkv * (ch < a.chunks ? ch : a.chunks);
   return s;
@@ -237,7 +237,7 @@ __device__ __forceinline__ int attend_plan(const AttendArgs& a, AttendPlan& p, i
     total += p.warp_sum[w];
   }
   int per = (total + a.workers - 1) / a.workers;
-  per = per < kAttendMinUnits ? kAttendMinUnits : per;
+  per = max(per, kAttendMinTok >> a.unit_log2);
 #pragma unroll
   for (int k = 0; k < kAttendWarps; ++k) {
     const int64_t u0 = (int64_t)(blockIdx.x * kAttendWarps + k) * per;
@@ -267,6 +267,7 @@ __device__ __forceinline__ float diff_value(float o1, float o2, float lam) { ret
 // Host side (paged_attend_mma.cu): the tensor-core kernel for these types and
 // shape; cols 8 or 16.  a == null only reports its resident CTAs in *grid.
 bool attend_mma_supported(int kv_dtype, int q_dtype, int D, int bs);
+int attend_mma_unit_log2(int kv_dtype, int D);
 int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid);
 
 }  // namespace clover

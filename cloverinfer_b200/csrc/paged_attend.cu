@@ -366,16 +366,6 @@ struct AppendRowsArgs {
   int32_t new_dtype, kv_dtype, n_rows;
 };
 
-template <bool FP8>
-__device__ __forceinline__ float encode_row_any(int dtype, const void* src, int64_t at, uint8_t* dst,
-                                                int D, int lane) {
-  switch (dtype) {
-    case CLOVER_B200_F32: return encode_row_warp<FP8>(static_cast<const float*>(src) + at, dst, D, lane);
-    case CLOVER_B200_F16: return encode_row_warp<FP8>(static_cast<const __half*>(src) + at, dst, D, lane);
-    default: return encode_row_warp<FP8>(static_cast<const __nv_bfloat16*>(src) + at, dst, D, lane);
-  }
-}
-
 __global__ void __launch_bounds__(256) attend_append_kernel(const AppendRowsArgs p) {
   const AttendArgs& a = p.a;
   const int lane = threadIdx.x & 31;
@@ -478,7 +468,7 @@ static int attend_generic(int kv_dtype, int D, int cols, const AttendArgs* a, cu
 
 struct AttendShape {
   bool mma, whole;
-  int cols, chunks, workers, sms;
+  int cols, chunks, workers, sms, unit_log2;
   int64_t part_bytes, ml_bytes, seg_bytes, bytes;
 };
 
@@ -511,20 +501,22 @@ static int attend_shape(int n_seqs, int n_rows, int max_q, int max_ctx, int hq, 
   p->cols = p->mma ? (cols > kMmaCols && D <= 128 ? 2 * kMmaCols : kMmaCols)
                    : cols >= 8 ? 8 : cols >= 4 ? 4 : cols >= 2 ? 2 : 1;
   const int64_t chunks = (cols + p->cols - 1) / p->cols;
-  const int64_t units = ((int64_t)max_ctx + kUnitTok - 1) / kUnitTok;
+  p->unit_log2 = p->mma ? attend_mma_unit_log2(kv_dtype, D) : 4;
+  const int64_t units = ((int64_t)max_ctx + (1 << p->unit_log2) - 1) >> p->unit_log2;
+  const int64_t least = kAttendMinTok >> p->unit_log2;  // units of a worker's least range
   if (chunks > 65535 || (int64_t)n_seqs * hkv * chunks > INT32_MAX / 64 ||
       (int64_t)n_seqs * hkv * chunks * (units > 0 ? units : 1) > INT32_MAX)
     return set_error(CLOVER_B200_ERR_UNSUPPORTED, "attend: batch too large");
   p->chunks = (int)chunks;
   // Short contexts: a segment is at most two ranges' least work; splitting it
   // would cost the second launch more than it gains.
-  p->whole = units <= 2 * kAttendMinUnits;
+  p->whole = units <= 2 * least;
   int grid = 0;
   const int rc = p->mma ? attend_mma(kv_dtype, q_dtype, p->cols, nullptr, D, nullptr, &grid)
                         : attend_generic(kv_dtype, D, p->cols, nullptr, nullptr, p->sms, &grid);
   if (rc) return rc;
   const int64_t segs = (int64_t)n_seqs * hkv * chunks;
-  const int64_t want = p->whole ? segs : (segs * units + kAttendMinUnits - 1) / kAttendMinUnits;
+  const int64_t want = p->whole ? segs : (segs * units + least - 1) / least;
   int64_t ctas = (want + kAttendWarps - 1) / kAttendWarps;
   if (ctas > grid) ctas = grid;
   if (ctas < 1) ctas = 1;
@@ -610,6 +602,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   a.bs = block_size;
   a.num_blocks = num_blocks;
   a.scale_log2 = score_scale * 1.4426950408889634f;
+  a.unit_log2 = sh.unit_log2;
   a.cols = sh.cols;
   a.chunks = sh.chunks;
   a.whole = sh.whole;
@@ -624,12 +617,17 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   a.norm_w = norm_weight;
   a.eps = eps;
   a.out_scale = out_scale;
-  // one fp16 weight term (2^-12) under a bf16 output, unless maps cancel
-  a.p_lo = 1;
   a.status = dev_status;
   a.wait_ns = wait_limit_ns();
   cudaStream_t s = (cudaStream_t)stream;
-  if (k_new) {
+  // With one chunk per (sequence, KV head) the worker that owns a new token's
+  // unit writes it before its copy; several chunks would read what one writes.
+  if (k_new && sh.mma && sh.chunks == 1) {
+    a.k_new = k_new;
+    a.v_new = v_new;
+    a.new_stride = new_token_stride;
+    a.new_dtype = new_dtype;
+  } else if (k_new) {
     AppendRowsArgs p{a, (uint8_t*)k_cache, (uint8_t*)v_cache, k_scales, v_scales, k_new, v_new,
                      new_token_stride, new_dtype, kv_dtype, n_query_rows};
     const int64_t want = ((int64_t)n_query_rows * 2 * num_kv_heads + 7) / 8;

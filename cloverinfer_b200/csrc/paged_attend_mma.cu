@@ -2,9 +2,10 @@
 // scales: head_dim 64, 128 or 256, block sizes that are multiples of 16.
 //
 // Each warp owns a ring of stages; a stage is one unit, 16 tokens of one KV
-// head: the K and V tiles (TMA, 128- or 64-byte swizzle) and, for 8 bits, the
-// 16 K and 16 V scales (two 64-byte bulk copies), one mbarrier for all.  Per
-// stage (tokens = M, columns = N = 8 per n-tile):
+// head (32 where a token row is at most 128 bytes): the K and V tiles (TMA
+// boxes of 16 tokens, 128- or 64-byte swizzle) and, for 8 bits, their K and V
+// scales (64-byte bulk copies), one mbarrier for all.  Per 16 tokens (tokens =
+// M, columns = N = 8 per n-tile):
 //     S[16 x 8] = K . Q^T,  O^T[D x 8] += V^T . P^T     (mma.sync m16n8k16)
 // tcgen05 would need 64 or 128 rows of M per instruction: a decode column tile
 // has 8 or 16 columns and every product here waits for memory, so the warp
@@ -25,10 +26,14 @@
 // weight times its scale is then at most 1, so fp16 holds it whatever the
 // scales are, and only one exponential is needed.  Weights are split into hi +
 // lo 16-bit terms (2^-16 of the weight in bf16, 2^-22 in fp16; three terms,
-// 2^-24, for fp32 queries over bf16).  One fp16 term, 2^-12, is used where the
-// output is bf16 (2^-9) and nothing cancels (one map).  fp32 queries are split
-// the same way; columns of fp16 products are first scaled by a power of two so
-// that their largest value is in [2^14, 2^15).
+// 2^-24, for fp32 queries over bf16).  fp32 queries are split the same way;
+// columns of fp16 products are first scaled by a power of two so that their
+// largest value is in [2^14, 2^15).
+//
+// The reference moves only when a stage's maximum exceeds it by more than 8
+// (weights then reach at most 2^8, far inside fp16 and fp32): with the running
+// maximum itself about half of the stages of a worker rescaled the
+// accumulators.
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -49,9 +54,10 @@ struct AttendGeom {
   static constexpr int kRow = D * kEsz;                  // bytes of a token row
   static constexpr int kSwz = kRow < 128 ? kRow : 128;   // bytes of a swizzled row
   static constexpr int kChunks = kRow / kSwz;            // TMA boxes per tile
-  static constexpr int kTile = kUnitTok * kRow;
+  static constexpr int kTok = kRow <= 128 ? 32 : 16;     // tokens of a unit
+  static constexpr int kTile = kTok * kRow;
   static constexpr int kTiles = 2 * kTile;               // K, V
-  static constexpr int kScales = kEight ? 2 * kUnitTok * 4 : 0;
+  static constexpr int kScales = kEight ? 2 * kTok * 4 : 0;
   static constexpr int kQTerms = !QF32 ? 1 : KV == KV_BF16 ? 3 : 2;
   static constexpr int kPTerms = KV == KV_BF16 && QF32 ? 3 : 2;
   // Accumulators and query fragments decide how many warps an SM's registers
@@ -71,9 +77,9 @@ struct AttendGeom {
 
 // Byte offset of 16-byte chunk c of tile row r (kSwz-byte rows, chunk groups
 // of kSwz bytes one after the other).
-template <int SWZ>
+template <int SWZ, int TOK>
 __device__ __forceinline__ uint32_t attend_swz(int r, int c) {
-  if (SWZ == 128) return (uint32_t)((c >> 3) * kUnitTok * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+  if (SWZ == 128) return (uint32_t)((c >> 3) * TOK * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
   return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
@@ -147,7 +153,7 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
   using T = typename KvMma<KV>::T;
   constexpr bool kNorm = G::kEight || (KV == KV_F16 && QF32);
   const int half = D / 2;
-  const int cap = cur.s.n * kUnitTok;
+  const int cap = cur.s.ctx;
   int least = cap;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -207,47 +213,47 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
   c.min_lim = __reduce_min_sync(0xffffffffu, least);
 }
 
-// Fragments of V^T for n-dims 16 dm .. 16 dm + 15 (two dm at once for 8 bits).
-template <int KV, int D>
+// Fragments of V^T, tokens 16 mt .. 16 mt + 15, for dims 16 i .. 16 i + 15 (8
+// bits: 32 i .. 32 i + 31, two M tiles).
+template <int KV, int SWZ, int TOK>
 struct VFrag {
   static constexpr int kPer = KV >= KV_I8 ? 2 : 1;
   uint32_t a[kPer][4];
-  __device__ __forceinline__ void load(uint32_t vs, int i, int lane) {
-    constexpr int SWZ = (D * (KV >= KV_I8 ? 1 : 2)) < 128 ? 64 : 128;
+  __device__ __forceinline__ void load(uint32_t vs, int mt, int i, int lane) {
     const int grp = lane >> 3;
     if (KV >= KV_I8) {
-      const int r = (lane & 7) + (grp & 1) * 8;
+      const int r = mt * 16 + (lane & 7) + (grp & 1) * 8;
       uint32_t x[4];
-      ldsm_x4_trans(vs + attend_swz<SWZ>(r, 2 * i + (grp >> 1)), x[0], x[1], x[2], x[3]);
+      ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp >> 1)), x[0], x[1], x[2], x[3]);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
         codes_to_f16<KV, true>(x[2 * k], a[k][0], a[k][1]);
         codes_to_f16<KV, true>(x[2 * k + 1], a[k][2], a[k][3]);
       }
     } else {
-      const int r = (lane & 7) + (grp >> 1) * 8;
-      ldsm_x4_trans(vs + attend_swz<SWZ>(r, 2 * i + (grp & 1)), a[0][0], a[0][1], a[0][2], a[0][3]);
+      const int r = mt * 16 + (lane & 7) + (grp >> 1) * 8;
+      ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp & 1)), a[0][0], a[0][1], a[0][2], a[0][3]);
     }
   }
 };
 
-// Zero V rows [r0, 16) of a stage.
-template <int ROW, int SWZ>
+// Zero V rows [r0, TOK) of a stage.
+template <int ROW, int SWZ, int TOK>
 __device__ __forceinline__ void zero_rows(uint8_t* v, int r0, int lane) {
   constexpr int kC = ROW / 16;
-  for (int i = lane; i < (kUnitTok - r0) * kC; i += 32)
-    *reinterpret_cast<uint4*>(v + attend_swz<SWZ>(r0 + i / kC, i % kC)) = make_uint4(0, 0, 0, 0);
+  for (int i = lane; i < (TOK - r0) * kC; i += 32)
+    *reinterpret_cast<uint4*>(v + attend_swz<SWZ, TOK>(r0 + i / kC, i % kC)) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();  // before the next copy into this slot
   __syncwarp();
 }
 
 // Whether rows [r0, r1) of a V tile hold an infinity or NaN (codes: e4m3 NaN).
-template <int KV, int ROW, int SWZ>
+template <int KV, int ROW, int SWZ, int TOK>
 __device__ __forceinline__ bool rows_nonfinite(const uint8_t* v, int r0, int r1, int lane) {
   constexpr int kC = ROW / 16;
   bool bad = false;
   for (int i = lane; i < (r1 - r0) * kC; i += 32) {
-    const uint4 x = *reinterpret_cast<const uint4*>(v + attend_swz<SWZ>(r0 + i / kC, i % kC));
+    const uint4 x = *reinterpret_cast<const uint4*>(v + attend_swz<SWZ, TOK>(r0 + i / kC, i % kC));
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -265,92 +271,97 @@ __device__ __forceinline__ bool rows_nonfinite(const uint8_t* v, int r0, int r1,
 
 // One stage of one warp.
 template <int KV, bool QF32, int D, int NT>
-__device__ __forceinline__ void attend_stage(const AttendArgs& a, uint32_t ks, uint32_t vs, uint8_t* vgen,
-                                             const float* scales, int tok0, int nvalid,
-                                             AttendCols<KV, QF32, D, NT>& c, int lane) {
+__device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, uint8_t* vgen, const float* scales,
+                                             int tok0, int nvalid, AttendCols<KV, QF32, D, NT>& c, int lane) {
   using G = AttendGeom<KV, QF32, D, NT>;
   using T = typename KvMma<KV>::T;
-  constexpr int KK = D / 16, QT = G::kQTerms, PT = G::kPTerms;
+  using VF = VFrag<KV, G::kSwz, G::kTok>;
+  constexpr int KK = D / 16, QT = G::kQTerms, PT = G::kPTerms, MT = G::kTok / 16;
+  constexpr int CH = MT * NT == 1 ? 2 : 1;  // independent chains per score tile
   const int g = lane >> 2;
 
-  // ---- S = K . Q^T, two chains per n-tile
-  float ch[NT][2][4];
+  // ---- S = K . Q^T, in base 2 with the scales, masked
+  float s[MT][NT][4];
+  float mx[NT][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) ch[nt][k][0] = ch[nt][k][1] = ch[nt][k][2] = ch[nt][k][3] = 0.f;
-  const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
-  if (G::kEight) {
+  for (int mt = 0; mt < MT; ++mt) {
+    float ch[NT][CH][4];
 #pragma unroll
-    for (int i = 0; i < KK / 2; ++i) {
-      uint32_t x[4];
-      ldsm_x4(ks + attend_swz<G::kSwz>(r, 2 * i + (lane >> 4)), x[0], x[1], x[2], x[3]);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < CH; ++k) ch[nt][k][0] = ch[nt][k][1] = ch[nt][k][2] = ch[nt][k][3] = 0.f;
+    const int r = mt * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+    if (G::kEight) {
+#pragma unroll
+      for (int i = 0; i < KK / 2; ++i) {
+        uint32_t x[4];
+        ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, 2 * i + (lane >> 4)), x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t a0, a1, a2, a3;
+          codes_to_f16<KV, false>(x[2 * k], a0, a2);
+          codes_to_f16<KV, false>(x[2 * k + 1], a1, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+              MmaOp<T>::run(ch[nt][k % CH], a0, a1, a2, a3, c.q[nt][2 * i + k][0][q], c.q[nt][2 * i + k][1][q]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
         uint32_t a0, a1, a2, a3;
-        codes_to_f16<KV, false>(x[2 * k], a0, a2);
-        codes_to_f16<KV, false>(x[2 * k + 1], a1, a3);
+        ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, kk * 2 + (lane >> 4)), a0, a1, a2, a3);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int q = 0; q < QT; ++q)
-            MmaOp<T>::run(ch[nt][k], a0, a1, a2, a3, c.q[nt][2 * i + k][0][q], c.q[nt][2 * i + k][1][q]);
+            MmaOp<T>::run(ch[nt][kk % CH], a0, a1, a2, a3, c.q[nt][kk][0][q], c.q[nt][kk][1][q]);
       }
     }
-  } else {
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      uint32_t a0, a1, a2, a3;
-      ldsm_x4(ks + attend_swz<G::kSwz>(r, kk * 2 + (lane >> 4)), a0, a1, a2, a3);
+    for (int h = 0; h < 2; ++h) {
+      const int row = mt * 16 + g + 8 * h, t = tok0 + row;
+      float ksc = 1.f, ve = 0.f;
+      if (G::kEight) {
+        ksc = scales[row];
+        // 2^ve >= V's scale; scales below 2^-110 count as that (2^-107 is the least stored)
+        ve = fmaxf((float)((int)(__float_as_uint(scales[G::kTok + row]) >> 23 & 255u) - 126), -110.f);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int q = 0; q < QT; ++q)
-          MmaOp<T>::run(ch[nt][kk & 1], a0, a1, a2, a3, c.q[nt][kk][0][q], c.q[nt][kk][1][q]);
+        for (int e = 0; e < 2; ++e) {
+          float raw = ch[nt][0][2 * h + e];
+          if (CH == 2) raw += ch[nt][CH - 1][2 * h + e];
+          raw *= c.sc[nt][e];
+          const float x = t < c.lim[nt][e] ? (G::kEight ? raw * ksc : raw) : -INFINITY;
+          s[mt][nt][2 * h + e] = x;
+          mx[nt][e] = fmaxf(mx[nt][e], G::kEight ? x + ve : x);
+        }
     }
   }
 
-  // ---- scale, mask, running maximum (of score + e for 8 bits)
-  float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f}, ve[2] = {0.f, 0.f};
-  if (G::kEight) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      ksc[h] = scales[g + 8 * h];
-      vsc[h] = scales[kUnitTok + g + 8 * h];
-      ve[h] = fmaxf((float)((int)(__float_as_uint(vsc[h]) >> 23 & 255u) - 126), -110.f);
-    }
-  }
-  float s[NT][4];
+  // ---- the reference: move it when a column outgrows it
   bool moved = false;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    float mx[2] = {-INFINITY, -INFINITY};
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = tok0 + g + 8 * h;
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float raw = (ch[nt][0][2 * h + e] + ch[nt][1][2 * h + e]) * c.sc[nt][e];
-        const float x = t < c.lim[nt][e] ? (G::kEight ? raw * ksc[h] : raw) : -INFINITY;
-        s[nt][2 * h + e] = x;
-        mx[e] = fmaxf(mx[e], G::kEight ? x + ve[h] : x);
-      }
+      for (int off = 4; off < 32; off <<= 1)
+        mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], off));
+      moved |= mx[nt][e] > c.m[nt][e] + 8.f;
     }
-#pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-      mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
-    }
-    moved |= mx[0] > c.m[nt][0] || mx[1] > c.m[nt][1];
-    ch[nt][0][0] = mx[0];
-    ch[nt][0][1] = mx[1];
-  }
   if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float nm = fmaxf(c.m[nt][e], ch[nt][0][e]);
+        const float nm = fmaxf(c.m[nt][e], mx[nt][e]);
         const float al = fast_exp2(c.m[nt][e] - (nm == -INFINITY ? 0.f : nm));
         c.m[nt][e] = nm;
         c.l[nt][e] *= al;
@@ -360,64 +371,59 @@ __device__ __forceinline__ void attend_stage(const AttendArgs& a, uint32_t ks, u
           c.acc[nt][i][2 + e] *= al;
         }
       }
-    }
   }
 
-  // ---- weights, split and transposed
-  uint32_t pt[NT][2][PT];
+  // Rows that some column does not see: past the context they are zeroed; a
+  // later token's infinity or NaN must not meet the zero weight of an earlier
+  // row (multi-token rows), so such a stage takes its columns limit by limit,
+  // zeroing rows as it goes.
+  bool plain = true;
+  if (KV != KV_I8 && tok0 + G::kTok > c.min_lim) {
+    if (nvalid < G::kTok) zero_rows<G::kRow, G::kSwz, G::kTok>(vgen, nvalid, lane);
+    const int lo = max(0, c.min_lim - tok0), hi = min(nvalid, G::kTok);
+    if (lo < hi && rows_nonfinite<KV, G::kRow, G::kSwz, G::kTok>(vgen, lo, hi, lane)) plain = false;
+  }
+
+  // ---- weights, split and transposed; O^T += V^T . P^T
+  uint32_t pt[MT][NT][2][PT];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float u0 = c.m[nt][0] == -INFINITY ? 0.f : c.m[nt][0];
-    const float u1 = c.m[nt][1] == -INFINITY ? 0.f : c.m[nt][1];
+  for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int t = tok0 + g + 8 * h;
-      float p0 = fast_exp2(s[nt][2 * h] - u0), p1 = fast_exp2(s[nt][2 * h + 1] - u1);
-      c.l[nt][0] += p0;
-      c.l[nt][1] += p1;
-      if (G::kEight) {  // (a masked token's scale may be anything)
-        p0 = t < c.lim[nt][0] ? p0 * vsc[h] : 0.f;
-        p1 = t < c.lim[nt][1] ? p1 * vsc[h] : 0.f;
-      }
-      split_terms<T, PT>(p0, p1, pt[nt][h]);
+      const int row = mt * 16 + g + 8 * h, t = tok0 + row;
+      const float vsc = G::kEight ? scales[G::kTok + row] : 1.f;
 #pragma unroll
-      for (int k = 0; k < PT; ++k) pt[nt][h][k] = movm_trans(pt[nt][h][k]);
-    }
-  }
-
-  // ---- O^T += V^T . P^T
-  constexpr int kPer = VFrag<KV, D>::kPer;
-  bool plain = true;
-  if (KV != KV_I8 && tok0 + kUnitTok > c.min_lim) {
-    // Rows that some column does not see: past the context they are zeroed; a
-    // later token's infinity or NaN must not meet the zero weight of an
-    // earlier row (multi-token rows), so such a stage takes its columns limit
-    // by limit, zeroing rows as it goes.
-    if (nvalid < kUnitTok) zero_rows<G::kRow, G::kSwz>(vgen, nvalid, lane);
-    const int lo = max(0, c.min_lim - tok0), hi = min(nvalid, kUnitTok);
-    if (lo < hi && rows_nonfinite<KV, G::kRow, G::kSwz>(vgen, lo, hi, lane)) plain = false;
-  }
-  if (plain) {
-#pragma unroll
-    for (int i = 0; i < KK / kPer; ++i) {
-      VFrag<KV, D> v;
-      v.load(vs, i, lane);
-#pragma unroll
-      for (int k = 0; k < kPer; ++k)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          MmaOp<T>::run(c.acc[nt][i * kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[nt][0][0],
-                        pt[nt][1][0]);
-          if (PT > 2 || a.p_lo) {
-#pragma unroll
-            for (int q = 1; q < PT; ++q)
-              MmaOp<T>::run(c.acc[nt][i * kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3],
-                            pt[nt][0][q], pt[nt][1][q]);
-          }
+      for (int nt = 0; nt < NT; ++nt) {
+        float p0 = fast_exp2(s[mt][nt][2 * h] - (c.m[nt][0] == -INFINITY ? 0.f : c.m[nt][0]));
+        float p1 = fast_exp2(s[mt][nt][2 * h + 1] - (c.m[nt][1] == -INFINITY ? 0.f : c.m[nt][1]));
+        c.l[nt][0] += p0;
+        c.l[nt][1] += p1;
+        if (G::kEight) {  // (a masked token's scale may be anything)
+          p0 = t < c.lim[nt][0] ? p0 * vsc : 0.f;
+          p1 = t < c.lim[nt][1] ? p1 * vsc : 0.f;
         }
+        split_terms<T, PT>(p0, p1, pt[mt][nt][h]);
+#pragma unroll
+        for (int k = 0; k < PT; ++k) pt[mt][nt][h][k] = movm_trans(pt[mt][nt][h][k]);
+      }
     }
-    return;
+    if (plain) {
+#pragma unroll
+      for (int i = 0; i < KK / VF::kPer; ++i) {
+        VF v;
+        v.load(vs, mt, i, lane);
+#pragma unroll
+        for (int k = 0; k < VF::kPer; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < PT; ++q)
+              MmaOp<T>::run(c.acc[nt][i * VF::kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3],
+                            pt[mt][nt][0][q], pt[mt][nt][1][q]);
+      }
+    }
   }
+  if (plain) return;
   for (int below = 0x7fffffff;;) {
     int top = 0;
 #pragma unroll
@@ -427,31 +433,70 @@ __device__ __forceinline__ void attend_stage(const AttendArgs& a, uint32_t ks, u
         if (c.lim[nt][e] < below) top = max(top, c.lim[nt][e]);
     top = __reduce_max_sync(0xffffffffu, top);
     if (top <= tok0) break;
-    if (top - tok0 < kUnitTok) zero_rows<G::kRow, G::kSwz>(vgen, top - tok0, lane);
+    if (top - tok0 < G::kTok) zero_rows<G::kRow, G::kSwz, G::kTok>(vgen, top - tok0, lane);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll 1
-    for (int i = 0; i < KK / kPer; ++i) {
-      VFrag<KV, D> v;
-      v.load(vs, i, lane);
+      for (int i = 0; i < KK / VF::kPer; ++i) {
+        VF v;
+        v.load(vs, mt, i, lane);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k)
+        for (int k = 0; k < VF::kPer; ++k)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int nt = 0; nt < NT; ++nt) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int q = 0; q < PT; ++q)
-            MmaOp<T>::run(x, v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[nt][0][q], pt[nt][1][q]);
-          // (constant indices: the accumulators stay in registers)
+            for (int q = 0; q < PT; ++q)
+              MmaOp<T>::run(x, v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[mt][nt][0][q], pt[mt][nt][1][q]);
+            // (constant indices: the accumulators stay in registers)
 #pragma unroll
-          for (int j = 0; j < KK; ++j) {
-            if (j != i * kPer + k) continue;
+            for (int j = 0; j < KK; ++j) {
+              if (j != i * VF::kPer + k) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c.lim[nt][e & 1] == top) c.acc[nt][j][e] += x[e];
+              for (int e = 0; e < 4; ++e)
+                if (c.lim[nt][e & 1] == top) c.acc[nt][j][e] += x[e];
+            }
           }
-        }
-    }
+      }
     below = top;
   }
+}
+
+// Fused append: the new tokens of the cursor's sequence that lie in its unit,
+// for KV head kvh, written before the unit is copied (slot[u]: first cache slot
+// of the unit's u-th 16 tokens).
+template <int KV, int D, int SUBS>
+__device__ __forceinline__ void append_unit(const AttendArgs& a, const Cursor& cur, int kvh,
+                                            const int (&slot)[SUBS], int lane) {
+  const int tok0 = cur.jj * SUBS * kUnitTok;
+  for (int j = 0; j < cur.s.nq; ++j) {
+    const int r = cur.s.row0 + j;
+    const int rel = __ldg(a.ctx + r) - 1 - tok0;
+    if (rel < 0 || rel >= SUBS * kUnitTok || rel + tok0 >= cur.s.ctx) continue;
+    const int base = SUBS == 1 || rel < kUnitTok ? slot[0] : slot[SUBS - 1];
+    const int64_t at = base + (rel & (kUnitTok - 1));
+    const int64_t row = (at * a.hkv + kvh) * D, src = (int64_t)r * a.new_stride + (int64_t)kvh * D;
+    if (KV >= KV_I8) {
+      uint8_t* kd = static_cast<uint8_t*>(const_cast<void*>(a.kc)) + row;
+      uint8_t* vd = static_cast<uint8_t*>(const_cast<void*>(a.vc)) + row;
+      const float ks = encode_row_any<KV == KV_E4M3>(a.new_dtype, a.k_new, src, kd, D, lane);
+      const float vs = encode_row_any<KV == KV_E4M3>(a.new_dtype, a.v_new, src, vd, D, lane);
+      const int64_t blk = at / a.bs, si = (blk * a.hkv + kvh) * a.bs + (at - blk * a.bs);
+      if (lane == 0) {
+        const_cast<float*>(a.ks)[si] = ks;
+        const_cast<float*>(a.vs)[si] = vs;
+      }
+    } else {
+      uint16_t* kd = static_cast<uint16_t*>(const_cast<void*>(a.kc)) + row;
+      uint16_t* vd = static_cast<uint16_t*>(const_cast<void*>(a.vc)) + row;
+      for (int d = lane; d < D; d += 32) {
+        kd[d] = static_cast<const uint16_t*>(a.k_new)[src + d];
+        vd[d] = static_cast<const uint16_t*>(a.v_new)[src + d];
+      }
+    }
+  }
+  fence_proxy_async_global();  // the copies read what was just written
+  __syncwarp();
 }
 
 template <int KV, bool QF32, int D, int NT>
@@ -517,54 +562,86 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (!more) return;
   Cursor cc = pc;  // the products' position
 
-  // Block ids of the copies' sequence, 32 at a time (lane i: block id_base + i).
-  int ids = -1, id_base = 0, id_b = -1;
-  const int upb = a.bs / kUnitTok;  // units per block
-  auto issue = [&](int k) {
-    const int bi = pc.jj / upb;
-    if (pc.b != id_b || bi < id_base || bi >= id_base + 32) {
-      id_b = pc.b;
-      id_base = bi;
+  // ---- copies.  Block ids of the sequence are held 32 at a time (lane i:
+  // block id_base + i); block and sub count 16-token steps of the segment.
+  constexpr int SUBS = G::kTok / kUnitTok;
+  const int upb = a.bs / kUnitTok;  // 16-token steps per block
+  int ids = 0, id_base = -64, p_b = -1, p_h = -1, p_kvh = 0, blk_i = 0, sub = 0, first_new = 0;
+  int p_st = 0;
+  auto issue = [&]() {
+    if (pc.b != p_b || pc.h != p_h) {
+      if (pc.b != p_b) id_base = -64;
+      p_b = pc.b;
+      p_h = pc.h;
+      p_kvh = pc.h / (pc.s.hc / a.hkv);
+      const int at = pc.jj * SUBS;
+      blk_i = at / upb;
+      sub = at - blk_i * upb;
+      if (a.k_new != nullptr) first_new = __ldg(a.ctx + pc.s.row0) - 1;
+    }
+    const int n_sub = (pc.s.ctx + kUnitTok - 1) / kUnitTok - pc.jj * SUBS;  // steps left
+    if (blk_i < id_base || blk_i + SUBS > id_base + 32) {
+      id_base = blk_i;
       const int trow = a.seq_rows ? __ldg(a.seq_rows + pc.b) : pc.b;
-      const int nblk = (pc.s.n + upb - 1) / upb;
+      const int nblk = (pc.s.ctx + a.bs - 1) / a.bs;
       ids = 0;
-      if (bi + lane < nblk) {
-        ids = bi + lane < a.table_stride ? __ldg(a.tables + (int64_t)trow * a.table_stride + bi + lane) : -1;
+      if (blk_i + lane < nblk) {
+        ids = blk_i + lane < a.table_stride
+                  ? __ldg(a.tables + (int64_t)trow * a.table_stride + blk_i + lane) : -1;
         if (ids < 0 || ids >= a.num_blocks) {
           raise_status(a.status, CLOVER_B200_DEV_BAD_BLOCK);
           ids = 0;  // keep the pipeline well-formed; the output is flagged
         }
       }
     }
-    const int blk = __shfl_sync(0xffffffffu, ids, bi - id_base);
-    if (lane == 0) {
-      const int off = (pc.jj - bi * upb) * kUnitTok;
-      const int kvh = pc.h / (pc.s.hc / a.hkv);
-      const int st = k % STAGES;
-      const uint32_t bar = bar0 + st * 8;
-      const uint32_t kd = ring_s + st * G::kTiles, vd = kd + G::kTile;
-      mbar_arrive_expect_tx(bar, G::kStageB);
+    int slot[SUBS];  // first cache slot of each 16-token step
+    int64_t sc_at[SUBS];
 #pragma unroll
-      for (int c = 0; c < G::kChunks; ++c) {
-        tma_load_3d(kd + c * kUnitTok * G::kSwz, &tmK, c * (G::kSwz / G::kEsz), kvh, blk * a.bs + off, bar);
-        tma_load_3d(vd + c * kUnitTok * G::kSwz, &tmV, c * (G::kSwz / G::kEsz), kvh, blk * a.bs + off, bar);
-      }
-      if (G::kEight) {
-        const int64_t at = ((int64_t)blk * a.hkv + kvh) * a.bs + off;
-        bulk_load(scales_s + st * G::kScales, a.ks + at, kUnitTok * 4, bar);
-        bulk_load(scales_s + st * G::kScales + kUnitTok * 4, a.vs + at, kUnitTok * 4, bar);
+    for (int u = 0; u < SUBS; ++u) {
+      const int blk = __shfl_sync(0xffffffffu, ids, blk_i - id_base);
+      slot[u] = blk * a.bs + sub * kUnitTok;
+      sc_at[u] = ((int64_t)blk * a.hkv + p_kvh) * a.bs + sub * kUnitTok;
+      if (++sub == upb) {
+        sub = 0;
+        ++blk_i;
       }
     }
+    if (a.k_new != nullptr && (pc.jj + 1) * G::kTok > first_new)
+      append_unit<KV, D>(a, pc, p_kvh, slot, lane);
+    const int subs = n_sub < SUBS ? n_sub : SUBS;
+    const uint32_t bar = bar0 + p_st * 8;
+    const uint32_t kd = ring_s + p_st * G::kTiles, vd = kd + G::kTile;
+    if (lane == 0) mbar_arrive_expect_tx(bar, subs * (G::kStageB / SUBS));
+    __syncwarp();
+    // one copy per lane: (step, K or V, chunk), then the scales
+    constexpr int kCopies = 2 * G::kChunks;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      if (u >= subs) break;
+      const int i = lane - u * (kCopies + 2);
+      if (i >= 0 && i < kCopies) {
+        const int ch = i >> 1;
+        tma_load_3d((i & 1 ? vd : kd) + (ch * G::kTok + u * kUnitTok) * G::kSwz, i & 1 ? &tmV : &tmK,
+                    ch * (G::kSwz / G::kEsz), p_kvh, slot[u], bar);
+      }
+      if (G::kEight && (i == kCopies || i == kCopies + 1)) {
+        const int v = i - kCopies;
+        bulk_load(scales_s + p_st * G::kScales + (v * G::kTok + u * kUnitTok) * 4, (v ? a.vs : a.ks) + sc_at[u],
+                  kUnitTok * 4, bar);
+      }
+    }
+    p_st = p_st + 1 == STAGES ? 0 : p_st + 1;
   };
 
   int issued = 0;
   while (issued < STAGES && more) {
-    issue(issued++);
+    issue();
+    ++issued;
     more = pc.next(a);
   }
 
   AttendCols<KV, QF32, D, NT> c;
-  int cur_b = -1, cur_h = -1, first_jj = 0, last_jj = 0, kvh = 0, chunk = 0, ctx_end = 0;
+  int cur_b = -1, cur_h = -1, first_jj = 0, last_jj = 0, kvh = 0, chunk = 0;
   Cursor seg = cc;  // the segment of the columns in registers
 
   auto finish = [&]() {
@@ -650,9 +727,9 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   };
 
   bool timed_out = false;
-  int k = 0;
+  int k = 0, st = 0;
+  uint32_t parity = 0;
   for (;; ++k) {
-    const int st = k % STAGES;
     if (cc.b != cur_b || cc.h != cur_h) {
       if (cur_b >= 0) finish();
       cur_b = cc.b;
@@ -662,22 +739,26 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int nch = cc.s.hc / a.hkv;
       kvh = cc.h / nch;
       chunk = cc.h - kvh * nch;
-      ctx_end = min(__ldg(a.ctx + cc.s.row0 + cc.s.nq - 1), a.max_ctx);
       load_columns<KV, QF32, D, NT>(a, cc, kvh, chunk, c, lane);
     }
-    if (!mbar_wait_bounded(bar0 + st * 8, (k / STAGES) & 1, a.wait_ns)) {
+    if (!mbar_wait_bounded(bar0 + st * 8, parity, a.wait_ns)) {
       timed_out = true;
       break;
     }
     last_jj = cc.jj;
-    const int tok0 = cc.jj * kUnitTok;
+    const int tok0 = cc.jj * G::kTok;
     const uint32_t ks = ring_s + st * G::kTiles;
-    attend_stage<KV, QF32, D, NT>(a, ks, ks + G::kTile, ring + st * G::kTiles + G::kTile,
-                                  scales + st * (G::kScales / 4), tok0, ctx_end - tok0, c, lane);
+    attend_stage<KV, QF32, D, NT>(ks, ks + G::kTile, ring + st * G::kTiles + G::kTile,
+                                  scales + st * (G::kScales / 4), tok0, cc.s.ctx - tok0, c, lane);
     __syncwarp();
     if (more) {
-      issue(issued++);
+      issue();
+      ++issued;
       more = pc.next(a);
+    }
+    if (++st == STAGES) {
+      st = 0;
+      parity ^= 1;
     }
     if (!cc.next(a)) break;
   }
@@ -731,7 +812,11 @@ static int attend_tmap(const void* ptr, int esz, int D, int H, int64_t slots, CU
   const CUresult r = encode(&e.map, esz == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
                             const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             swz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            // a token row at most: its neighbours are other heads' rows
+                            row >= 256   ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                            : row == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                         : CU_TENSOR_MAP_L2_PROMOTION_L2_64B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(CLOVER_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   cache[next] = e;
   next = (next + 1) % 64;
@@ -790,6 +875,11 @@ static int mma_shape(int cols, const AttendArgs* a, int D, cudaStream_t s, int* 
 
 bool attend_mma_supported(int kv_dtype, int q_dtype, int D, int bs) {
   return (D == 64 || D == 128 || D == 256) && bs % kUnitTok == 0 && kv_dtype != CLOVER_B200_F32;
+}
+
+int attend_mma_unit_log2(int kv_dtype, int D) {
+  const bool eight = kv_dtype == CLOVER_B200_INT8 || kv_dtype == CLOVER_B200_FP8_E4M3;
+  return D * (eight ? 1 : 2) <= 128 ? 5 : 4;
 }
 
 int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid) {

@@ -75,4 +75,15 @@ __device__ __forceinline__ float encode_row_warp(const TI* src, uint8_t* dst, in
   return s;
 }
 
+// The same for a row of any type at element `at` of src.
+template <bool FP8>
+__device__ __forceinline__ float encode_row_any(int dtype, const void* src, int64_t at, uint8_t* dst,
+                                                int D, int lane) {
+  switch (dtype) {
+    case CLOVER_B200_F32: return encode_row_warp<FP8>(static_cast<const float*>(src) + at, dst, D, lane);
+    case CLOVER_B200_F16: return encode_row_warp<FP8>(static_cast<const __half*>(src) + at, dst, D, lane);
+    default: return encode_row_warp<FP8>(static_cast<const __nv_bfloat16*>(src) + at, dst, D, lane);
+  }
+}
+
 }  // namespace clover
