@@ -7,15 +7,23 @@
 // n = ceil(ctx_b / unit) units, ctx_b the context of the sequence's last row (rows are in causal
 // order).  A column is one (query row, query head of the KV head's group,
 // map), so a KV tile is read once for all heads of a group, all new tokens and
-// both maps.  A worker is one warp.
-//   * split launches: units are numbered sequence-major, then segment, then
-//     along the context, and worker w takes [w per, (w + 1) per), so ragged
-//     batches leave no worker idle.  A worker's range meets at most two
-//     segments it does not hold whole: its first (a piece that starts inside
+// both maps.  A worker is one warp (generic kernel) or one ring of stages with
+// its warps (tensor-core kernel).
+//   * aligned launches: a segment is cut into ceil(n / per) equal pieces, per
+//     the least range for which the step has at most as many pieces as there
+//     are workers; pieces are numbered sequence-major, then along the context,
+//     then by segment, and worker w takes piece w (partial slot w).  The heads of
+//     a KV block then stream at the same time, so DRAM serves whole blocks
+//     instead of one head's 128 or 256 bytes here and there.
+//   * ranged launches, where aligned pieces would leave workers idle (more
+//     than a sixth longer than an even share: many segments, or very ragged
+//     ones): units are numbered sequence-major, then segment, then along the
+//     context, and worker w takes [w per, (w + 1) per).  A range meets at most
+//     two segments it does not hold whole: its first (a piece that starts inside
 //     the segment, partial slot 2w) and its last (a piece with the segment's
-//     first unit, slot 2w + 1).  The workspace is therefore 2 slots per worker
-//     whatever the batch, and the pieces of a segment are slot 2w + 1 of its
-//     first worker and slots 2(w + 1), 2(w + 2), ... of the following ones.
+//     first unit, slot 2w + 1).  The workspace is 2 slots per worker whatever
+//     the batch, and the pieces of a segment are slot 2w + 1 of its first worker
+//     and slots 2(w + 1), 2(w + 2), ... of the following ones.
 //   * whole launches (short contexts): worker w takes segments w, w + W, ...
 //     and writes their outputs; no second kernel runs.
 #pragma once
@@ -28,10 +36,10 @@
 namespace clover {
 
 constexpr int kUnitTok = 16;     // a unit is a multiple of this
-constexpr int kAttendWarps = 4;  // workers of a CTA
+constexpr int kAttendWarps = 4;  // workers of a generic CTA
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kAttendMinTok = 128;  // a worker's least range
-constexpr int kAttendMaxPerSm = 16; // workers per SM the workspace allows for
+constexpr int kAttendMaxPerSm = 16; // generic workers per SM
 
 struct AttendArgs {
   void* out;
@@ -61,7 +69,9 @@ struct AttendArgs {
   // workspace of split launches
   float* part;    // [2 workers][cols][D]: unnormalised outputs
   float2* part_ml;  // [2 workers][cols]: running maximum (base 2) and sum
-  int2* seg;      // [n_seqs][hkv][chunks]: first worker and number of pieces
+  // [n_seqs][hkv][chunks]: the segment's pieces are slots x, y + z, y + 2z, ...
+  // (w of them; <= 1: written by its worker)
+  int4* seg;
   // differential attention
   const float* lam;
   const float* norm_w;
@@ -151,21 +161,13 @@ __device__ __forceinline__ void attend_check_seq(const AttendArgs& a, const SeqI
 }
 
 // A worker's position: unit jj of segment h (of s.hc) of sequence b; seg0 is the
-// flat number of the segment's first unit.  Split launches end after `left`
-// units, whole launches at the last segment.
+// flat number of the segment's first unit (ranged launches) or the segment
+// (whole ones).  Aligned and ranged launches end after `left` units, whole ones
+// at the last segment.
 struct Cursor {
   int b, h, jj, left, seg0;
   SeqInfo s;
 
-  // The first unit of a worker (b, offset of its first unit within b).
-  __device__ __forceinline__ void start(const AttendArgs& a, int b0, int off, int base, int units) {
-    b = b0;
-    s = seq_info(a, b);
-    h = off / s.n;
-    jj = off - h * s.n;
-    seg0 = base + h * s.n;
-    left = units;
-  }
   // Whole launches: the first segment with units among sg, sg + workers, ...
   __device__ __forceinline__ bool seek(const AttendArgs& a, int64_t sg) {
     const int hcmax = a.hkv * a.chunks;
@@ -201,24 +203,74 @@ struct Cursor {
   }
 };
 
-// Shared memory of the plan.
+// Shared memory of the plan of a CTA with NW warps and R workers.
+constexpr int kAlignTries = 6;  // aligned ranges up to 5/32 longer than an even share
+template <int NW, int R>
 struct AttendPlan {
-  int warp_sum[kAttendWarps];
-  int start[kAttendWarps][3];  // sequence, offset in it, flat number of its first unit
+  int sum[NW][kAlignTries + 1];  // per warp: units, then pieces at each range tried
+  int start[R][4];               // sequence, segment, first unit, units (ranged: flat number of the segment)
+  int seg0[R];
+};
+
+// What all workers of a launch share: units per worker, and whether the pieces
+// are aligned.
+struct AttendSplit {
+  int per, total;
+  bool aligned;
 };
 
 // Every CTA counts the step's units by itself (thread i takes sequences
-// [i c, (i + 1) c)) and finds where its workers start.  Returns the units per
-// worker; all threads call it.
-__device__ __forceinline__ int attend_plan(const AttendArgs& a, AttendPlan& p, int& total) {
+// [i c, (i + 1) c)) and finds where its workers (r * gridDim.x + blockIdx.x)
+// start; all threads call it.
+template <int NW, int R>
+__device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPlan<NW, R>& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int c = (a.n_seqs + kAttendThreads - 1) / kAttendThreads;
-  const int b0 = tid * c, b1 = min(a.n_seqs, b0 + c);
+  const int c = (a.n_seqs + NW * 32 - 1) / (NW * 32);
+  const int b0 = min(a.n_seqs, tid * c), b1 = min(a.n_seqs, b0 + c);
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     const SeqInfo s = seq_info(a, b);
     if (blockIdx.x == 0) attend_check_seq(a, s);
     mine += s.n * s.hc;
+  }
+  int x = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) p.sum[warp][0] = x;
+  if (tid < R) p.start[tid][0] = -1;
+  __syncthreads();
+  AttendSplit sp{0, 0, false};
+#pragma unroll
+  for (int w = 0; w < NW; ++w) sp.total += p.sum[w][0];
+  const int even = max((sp.total + a.workers - 1) / a.workers, kAttendMinTok >> a.unit_log2);
+  int pieces[kAlignTries];
+#pragma unroll
+  for (int k = 0; k < kAlignTries; ++k) pieces[k] = 0;
+  for (int b = b0; b < b1; ++b) {
+    const SeqInfo s = seq_info(a, b);
+#pragma unroll
+    for (int k = 0; k < kAlignTries; ++k) {
+      const int per = even + (even * k + 31) / 32;
+      pieces[k] += s.hc * ((s.n + per - 1) / per);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kAlignTries; ++k) {
+    x = __reduce_add_sync(0xffffffffu, pieces[k]);
+    if (lane == 0) p.sum[warp][k + 1] = x;
+  }
+  __syncthreads();
+  int col = 0;  // of p.sum: what is numbered
+  sp.per = even;
+#pragma unroll
+  for (int k = 0; k < kAlignTries; ++k) {
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += p.sum[w][k + 1];
+    if (!sp.aligned && all <= a.workers) {
+      sp.aligned = true;
+      sp.per = even + (even * k + 31) / 32;
+      mine = pieces[k];
+      col = k + 1;
+    }
   }
   int incl = mine;
 #pragma unroll
@@ -226,38 +278,72 @@ __device__ __forceinline__ int attend_plan(const AttendArgs& a, AttendPlan& p, i
     const int y = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += y;
   }
-  if (lane == 31) p.warp_sum[warp] = incl;
-  if (tid < kAttendWarps) p.start[tid][0] = -1;
-  __syncthreads();
   int before = incl - mine;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kAttendWarps; ++w) {
-    if (w < warp) before += p.warp_sum[w];
-    total += p.warp_sum[w];
-  }
-  int per = (total + a.workers - 1) / a.workers;
-  per = max(per, kAttendMinTok >> a.unit_log2);
-#pragma unroll
-  for (int k = 0; k < kAttendWarps; ++k) {
-    const int64_t u0 = (int64_t)(blockIdx.x * kAttendWarps + k) * per;
-    if (u0 >= before && u0 < before + mine) {
-      int at = before;
-      for (int b = b0; b < b1; ++b) {
-        const SeqInfo s = seq_info(a, b);
-        const int u = s.n * s.hc;
-        if (u0 < at + u) {
-          p.start[k][0] = b;
-          p.start[k][1] = (int)(u0 - at);
-          p.start[k][2] = at;
-          break;
+  for (int w = 0; w < warp; ++w) before += p.sum[w][col];
+  for (int k = 0; k < R; ++k) {
+    const int wid = k * gridDim.x + blockIdx.x;
+    const int64_t u0 = sp.aligned ? wid : (int64_t)wid * sp.per;
+    if (u0 < before || u0 >= before + mine) continue;
+    int at = before;
+    for (int b = b0; b < b1; ++b) {
+      const SeqInfo s = seq_info(a, b);
+      const int kp = (s.n + sp.per - 1) / sp.per;
+      const int u = s.hc * (sp.aligned ? kp : s.n);
+      if (u0 < at + u) {
+        const int off = (int)(u0 - at);
+        p.start[k][0] = b;
+        if (sp.aligned) {
+          const int i = off / s.hc, len = (s.n + kp - 1) / kp;
+          p.start[k][1] = off - i * s.hc;
+          p.start[k][2] = i * len;
+          p.start[k][3] = min(len, s.n - i * len);
+          p.seg0[k] = 0;
+          if (i * len >= s.n) p.start[k][0] = -1;  // (rounding left the last piece empty)
+        } else {
+          const int h = off / s.n;
+          p.start[k][1] = h;
+          p.start[k][2] = off - h * s.n;
+          p.start[k][3] = (int)min((int64_t)sp.per, sp.total - u0);
+          p.seg0[k] = at + h * s.n;
         }
-        at += u;
+        break;
       }
+      at += u;
     }
   }
   __syncthreads();
-  return per;
+  return sp;
+}
+
+// Worker r's first unit; false without one.
+template <int NW, int R>
+__device__ __forceinline__ bool attend_start(const AttendArgs& a, const AttendPlan<NW, R>& p, int r, Cursor& cur) {
+  if (p.start[r][0] < 0) return false;
+  cur.b = p.start[r][0];
+  cur.s = seq_info(a, cur.b);
+  cur.h = p.start[r][1];
+  cur.jj = p.start[r][2];
+  cur.left = p.start[r][3];
+  cur.seg0 = p.seg0[r];
+  return true;
+}
+
+// The partial slot of a worker's piece, and (from the piece with the segment's
+// first unit) the segment's entry for the join.
+__device__ __forceinline__ int64_t attend_slot(const AttendSplit& sp, int wid, int first_jj) {
+  return sp.aligned ? wid : 2 * (int64_t)wid + (first_jj == 0 ? 1 : 0);
+}
+__device__ __forceinline__ void attend_record(const AttendArgs& a, const AttendSplit& sp, int b, int h, int seg0,
+                                              const SeqInfo& s, int wid) {
+  int4 e;
+  if (sp.aligned) {
+    const int kp = (s.n + sp.per - 1) / sp.per, len = (s.n + kp - 1) / kp;
+    e = make_int4(wid, wid, s.hc, (s.n + len - 1) / len);
+  } else {
+    const int fw = seg0 / sp.per;
+    e = make_int4(2 * fw + 1, 2 * fw, 2, (seg0 + s.n - 1) / sp.per - fw + 1);
+  }
+  a.seg[(int64_t)b * (a.hkv * a.chunks) + h] = e;
 }
 
 // ------------------------------------------------------------------ results
@@ -265,9 +351,10 @@ __device__ __forceinline__ int attend_plan(const AttendArgs& a, AttendPlan& p, i
 __device__ __forceinline__ float diff_value(float o1, float o2, float lam) { return fmaf(-lam, o2, o1); }
 
 // Host side (paged_attend_mma.cu): the tensor-core kernel for these types and
-// shape; cols 8 or 16.  a == null only reports its resident CTAs in *grid.
+// shape; cols 8 or 16.  a == null only reports its most CTAs and the workers of
+// one.
 bool attend_mma_supported(int kv_dtype, int q_dtype, int D, int bs);
 int attend_mma_unit_log2(int kv_dtype, int D);
-int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid);
+int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid, int* rings);
 
 }  // namespace clover

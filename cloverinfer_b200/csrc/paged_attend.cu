@@ -37,21 +37,18 @@ __device__ __forceinline__ float load_cache<__nv_fp8_e4m3>(const __nv_fp8_e4m3* 
 template <typename KT, int EPL, int NC>
 __global__ void __launch_bounds__(kAttendThreads)
 attend_generic_kernel(const AttendArgs a) {
-  __shared__ AttendPlan plan;
+  __shared__ AttendPlan<kAttendWarps, kAttendWarps> plan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int wid = blockIdx.x * kAttendWarps + warp;
+  const int wid = warp * gridDim.x + blockIdx.x;
   pdl_wait();
-  int per = 0, total = 0;
+  AttendSplit sp{1, 0, false};
   Cursor cur;
   int seg = 0;  // whole launches: the worker's segment (empty ones too: their zeros)
   const int hcmax = a.hkv * a.chunks;
   if (!a.whole) {
-    per = attend_plan(a, plan, total);
+    sp = attend_plan<kAttendWarps, kAttendWarps>(a, plan);
     pdl_trigger();
-    const int64_t u0 = (int64_t)wid * per;
-    if (u0 >= total || plan.start[warp][0] < 0) return;
-    cur.start(a, plan.start[warp][0], plan.start[warp][1], plan.start[warp][2],
-              (int)min((int64_t)per, total - u0));
+    if (!attend_start(a, plan, warp, cur)) return;
   } else {
     seg = wid - a.workers;
   }
@@ -104,7 +101,8 @@ attend_generic_kernel(const AttendArgs a) {
     const int trow = a.seq_rows ? __ldg(a.seq_rows + cur.b) : cur.b;
     const int32_t* tab = a.tables + (int64_t)trow * a.table_stride;
     const int ctx_end = min(__ldg(a.ctx + cur.s.row0 + cur.s.nq - 1), a.max_ctx);
-    const int b = cur.b, h = cur.h, n = cur.s.n, seg0 = cur.seg0, row0 = cur.s.row0, nq = cur.s.nq;
+    const SeqInfo seq = cur.s;
+    const int b = cur.b, h = cur.h, n = seq.n, seg0 = cur.seg0, row0 = seq.row0, nq = seq.nq;
     int last_jj = -1;
     bool more = true;
     while (cur.left > 0 && more && cur.b == b && cur.h == h) {
@@ -190,7 +188,7 @@ attend_generic_kernel(const AttendArgs a) {
     // ---- the piece is done: the output, or a partial
     const bool is_whole = a.whole || (first_jj == 0 && last_jj == n - 1);
     if (!is_whole) {
-      const int64_t slot = 2 * (int64_t)wid + (first_jj == 0 ? 1 : 0);
+      const int64_t slot = attend_slot(sp, wid, first_jj);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
 #pragma unroll
@@ -232,10 +230,7 @@ attend_generic_kernel(const AttendArgs a) {
           if (lane + 32 * e < a.D) attend_store(a, ob + lane + 32 * e, o[e]);
       }
     }
-    if (!a.whole && first_jj == 0 && lane == 0) {
-      const int first_w = seg0 / per;
-      a.seg[(int64_t)b * hcmax + h] = make_int2(first_w, (seg0 + n - 1) / per - first_w + 1);
-    }
+    if (!a.whole && first_jj == 0 && lane == 0) attend_record(a, sp, b, h, seg0, seq, wid);
     if (!a.whole && (!more || cur.left <= 0)) break;
   }
 }
@@ -272,17 +267,18 @@ attend_join_kernel(const AttendArgs a, int n_units) {
       for (int d = tid; d < a.D; d += kJoinThreads) attend_store(a, ob + d, 0.f);
       continue;
     }
-    const int2 sg = a.seg[seg];
-    if (sg.y <= 1) continue;  // written by its worker
+    const int4 sg = a.seg[seg];
+    if (sg.w <= 1) continue;  // written by its worker
     // (a worker that gave up waiting leaves its segment's entry unwritten)
-    if (sg.x < 0 || sg.x >= a.workers || sg.y > a.workers - sg.x) continue;
+    const int64_t last = sg.y + (int64_t)(sg.w - 1) * sg.z;
+    if (sg.x < 0 || sg.y < 0 || sg.z <= 0 || sg.x >= 2 * a.workers || last >= 2 * a.workers) continue;
     const int lim = ci.lim;
     for (int mp = 0; mp < a.maps; ++mp) {
       float m = -INFINITY, l = 0.f, o[EPL];
 #pragma unroll
       for (int e = 0; e < EPL; ++e) o[e] = 0.f;
-      for (int i = warp; i < sg.y; i += kJoinWarps) {
-        const int64_t slot = 2 * (int64_t)(sg.x + i) + (i == 0 ? 1 : 0);
+      for (int i = warp; i < sg.w; i += kJoinWarps) {
+        const int64_t slot = i == 0 ? sg.x : sg.y + (int64_t)i * sg.z;
         const int64_t at = slot * a.cols + c0 + mp;
         const float2 ml = __ldcg(a.part_ml + at);
         float x[EPL];
@@ -498,7 +494,7 @@ static int attend_shape(int n_seqs, int n_rows, int max_q, int max_ctx, int hq, 
     cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev);
   const int64_t cols = (int64_t)max_q * (hq / hkv) * maps;
   p->mma = attend_mma_supported(kv_dtype, q_dtype, D, bs);
-  p->cols = p->mma ? (cols > kMmaCols && D <= 128 ? 2 * kMmaCols : kMmaCols)
+  p->cols = p->mma ? (cols > kMmaCols ? 2 * kMmaCols : kMmaCols)
                    : cols >= 8 ? 8 : cols >= 4 ? 4 : cols >= 2 ? 2 : 1;
   const int64_t chunks = (cols + p->cols - 1) / p->cols;
   p->unit_log2 = p->mma ? attend_mma_unit_log2(kv_dtype, D) : 4;
@@ -511,21 +507,20 @@ static int attend_shape(int n_seqs, int n_rows, int max_q, int max_ctx, int hq, 
   // Short contexts: a segment is at most two ranges' least work; splitting it
   // would cost the second launch more than it gains.
   p->whole = units <= 2 * least;
-  int grid = 0;
-  const int rc = p->mma ? attend_mma(kv_dtype, q_dtype, p->cols, nullptr, D, nullptr, &grid)
+  int grid = 0, rings = kAttendWarps;
+  const int rc = p->mma ? attend_mma(kv_dtype, q_dtype, p->cols, nullptr, D, nullptr, &grid, &rings)
                         : attend_generic(kv_dtype, D, p->cols, nullptr, nullptr, p->sms, &grid);
   if (rc) return rc;
   const int64_t segs = (int64_t)n_seqs * hkv * chunks;
   const int64_t want = p->whole ? segs : (segs * units + least - 1) / least;
-  int64_t ctas = (want + kAttendWarps - 1) / kAttendWarps;
-  if (ctas > grid) ctas = grid;
-  if (ctas < 1) ctas = 1;
-  p->workers = (int)ctas * kAttendWarps;
+  // one CTA per worker until every CTA has one: few workers spread over the SMs
+  const int64_t ctas = want < 1 ? 1 : want < grid ? want : grid;
+  p->workers = (int)ctas * rings;
   p->part_bytes = p->ml_bytes = p->seg_bytes = 0;
   if (!p->whole) {
     p->part_bytes = round256(2ll * p->workers * p->cols * D * 4);
     p->ml_bytes = round256(2ll * p->workers * p->cols * 8);
-    p->seg_bytes = round256(segs * 8);
+    p->seg_bytes = round256(segs * 16);
   }
   p->bytes = p->part_bytes + p->ml_bytes + p->seg_bytes;
   return CLOVER_B200_OK;
@@ -611,7 +606,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   if (!sh.whole) {
     a.part = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + sh.part_bytes);
-    a.seg = reinterpret_cast<int2*>(ws + sh.part_bytes + sh.ml_bytes);
+    a.seg = reinterpret_cast<int4*>(ws + sh.part_bytes + sh.ml_bytes);
   }
   a.lam = lam;
   a.norm_w = norm_weight;
@@ -636,7 +631,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
     rc = check_cuda(cudaGetLastError(), "attend_append launch");
     if (rc) return rc;
   }
-  rc = sh.mma ? attend_mma(kv_dtype, q_dtype, sh.cols, &a, head_dim, s, nullptr)
+  rc = sh.mma ? attend_mma(kv_dtype, q_dtype, sh.cols, &a, head_dim, s, nullptr, nullptr)
               : attend_generic(kv_dtype, head_dim, sh.cols, &a, s, sh.sms, nullptr);
   if (rc || sh.whole) return rc;
   const int64_t units = (int64_t)n_seqs * num_kv_heads * sh.chunks * (sh.cols / maps);

@@ -1,14 +1,21 @@
 // Tensor-core decode over a 16-bit cache (differential) or an 8-bit cache with
 // scales: head_dim 64, 128 or 256, block sizes that are multiples of 16.
 //
-// Each warp owns a ring of stages; a stage is one unit, 16 tokens of one KV
-// head (32 where a token row is at most 128 bytes): the K and V tiles (TMA
-// boxes of 16 tokens, 128- or 64-byte swizzle) and, for 8 bits, their K and V
-// scales (64-byte bulk copies), one mbarrier for all.  Per 16 tokens (tokens =
-// M, columns = N = 8 per n-tile):
+// One CTA per SM.  A ring of stages belongs to CW warps ("column warps": CW = 1
+// for up to 8 columns of a chunk, 2 for 16), which read the same stages, each
+// for its own 8 columns; a ring with its warps is a worker of
+// attend_common.cuh.  A stage is one unit, 16 tokens of one KV head (32 where a
+// token row is at most 128 bytes): the K and V tiles (TMA boxes of 16 tokens,
+// 128- or 64-byte swizzle) and, for 8 bits, their scales (16 bytes per lane,
+// cp.async), all completing on one mbarrier.  The ring's first warp refills a
+// stage when it is done with it.  Two other ways were measured at 8 x 32k
+// tokens, e4m3: one warp that issues for all rings (165 us with the scales as
+// bulk copies, 179 as here: its own instructions are the limit), and the scales
+// as bulk copies (half of all copies for 6 % of the bytes).
+// Per 16 tokens (tokens = M, columns = N = 8):
 //     S[16 x 8] = K . Q^T,  O^T[D x 8] += V^T . P^T     (mma.sync m16n8k16)
 // tcgen05 would need 64 or 128 rows of M per instruction: a decode column tile
-// has 8 or 16 columns and every product here waits for memory, so the warp
+// has 8 columns and every product here waits for memory, so the warp
 // instruction on fragments in registers is the right size.
 //
 // 8-bit codes become fp16 in registers, exactly, between ldmatrix and the
@@ -22,18 +29,18 @@
 //   * int8: byte ^ 0x80 under 0x64 is the fp16 1024 + 128 + x; subtract 1152.
 //     e4m3: the conversion instruction.
 // K's scale multiplies the score; V's scale multiplies the softmax weight.  The
-// weights' reference is the running maximum of score + e, 2^e >= V's scale: a
-// weight times its scale is then at most 1, so fp16 holds it whatever the
-// scales are, and only one exponential is needed.  Weights are split into hi +
-// lo 16-bit terms (2^-16 of the weight in bf16, 2^-22 in fp16; three terms,
-// 2^-24, for fp32 queries over bf16).  fp32 queries are split the same way;
-// columns of fp16 products are first scaled by a power of two so that their
-// largest value is in [2^14, 2^15).
+// weights' reference is a bound of score + e, 2^e >= V's scale: a weight times
+// its scale is then bounded, so fp16 holds it whatever the scales are, and only
+// one exponential is needed.  Weights are split into hi + lo 16-bit terms (2^-16
+// of the weight in bf16, 2^-22 in fp16; three terms, 2^-24, for fp32 queries
+// over bf16).  fp32 queries are split the same way; columns of fp16 products are
+// first scaled by a power of two so that their largest value is in
+// [2^14, 2^15).
 //
-// The reference moves only when a stage's maximum exceeds it by more than 8
-// (weights then reach at most 2^8, far inside fp16 and fp32): with the running
-// maximum itself about half of the stages of a worker rescaled the
-// accumulators.
+// The reference moves only when a weight exceeds it by more than 2^8 (far inside
+// fp16 and fp32): with the running maximum itself about half of the stages of a
+// worker rescaled the accumulators, and every stage took the columns' maxima
+// over the lanes.
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -47,36 +54,43 @@ enum { KV_BF16 = 0, KV_F16 = 1, KV_I8 = 2, KV_E4M3 = 3 };
 template <int KV> struct KvMma { using T = __half; };
 template <> struct KvMma<KV_BF16> { using T = __nv_bfloat16; };
 
-template <int KV, bool QF32, int D, int NT>
+constexpr bool attend_fits(int rings, int stage, int budget) { return rings * 2 * stage <= budget; }
+
+template <int KV, bool QF32, int D, int CW_>
 struct AttendGeom {
+  static constexpr int CW = CW_;
   static constexpr bool kEight = KV >= KV_I8;
   static constexpr int kEsz = kEight ? 1 : 2;
   static constexpr int kRow = D * kEsz;                  // bytes of a token row
   static constexpr int kSwz = kRow < 128 ? kRow : 128;   // bytes of a swizzled row
-  static constexpr int kChunks = kRow / kSwz;            // TMA boxes per tile
+  static constexpr int kChunks = kRow / kSwz;            // TMA boxes per 16 tokens
   static constexpr int kTok = kRow <= 128 ? 32 : 16;     // tokens of a unit
+  static constexpr int kSubs = kTok / kUnitTok;
   static constexpr int kTile = kTok * kRow;
   static constexpr int kTiles = 2 * kTile;               // K, V
   static constexpr int kScales = kEight ? 2 * kTok * 4 : 0;
+  static constexpr int kStageB = kTiles + kScales;
   static constexpr int kQTerms = !QF32 ? 1 : KV == KV_BF16 ? 3 : 2;
   static constexpr int kPTerms = KV == KV_BF16 && QF32 ? 3 : 2;
-  // Accumulators and query fragments decide how many warps an SM's registers
-  // hold (4, 3 or 2 CTAs of 4 warps); the ring takes what shared memory that
-  // leaves, at least two stages where they fit.
-  static constexpr int kRegs = D / 16 * NT * (4 + 2 * kQTerms) + 64;
-  static constexpr int kWantCtas = kRegs <= 128 ? 4 : kRegs <= 168 ? 3 : 2;
-  static constexpr int kBudget = 216 * 1024;
-  static constexpr int kStageB = kTiles + kScales;
-  static constexpr int kCtas =
-      kWantCtas == 4 && 4 * (kAttendWarps * 2 * kStageB + 1024) > kBudget ? 3 : kWantCtas;
-  static constexpr int kFit = (kBudget / kCtas - 1024) / (kAttendWarps * kStageB);
+  // Warps: 16, 12 or 8 (128, 168 or 255 registers each), as many as hold
+  // accumulators, query fragments and about 80 more, with rings at least two
+  // stages deep.
+  static constexpr int kRegs = D / 4 + D / 8 * kQTerms + (kEight ? 92 : 80);
+  static constexpr int kBudget = 232448 - 1024 - 1024;  // an SM's shared memory, less alignment and barriers
+  static constexpr int kWarps = kRegs <= 128 && attend_fits(16 / CW, kStageB, kBudget)   ? 16
+                                : kRegs <= 180 && attend_fits(12 / CW, kStageB, kBudget) ? 12
+                                : attend_fits(8 / CW, kStageB, kBudget)                  ? 8
+                                                                                         : 6;
+  static constexpr int kRings = kWarps / CW;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kFit = kBudget / (kRings * kStageB);
   static constexpr int kStages = kFit < 1 ? 1 : kFit > 8 ? 8 : kFit;
-  static constexpr int kWarpTiles = kStages * kTiles;
-  static constexpr int kSmem = kAttendWarps * kStages * kStageB + 1024;
+  static constexpr int kRingTiles = kStages * kTiles;
+  static constexpr int kSmem = kRings * kStages * kStageB + 1024;
 };
 
-// Byte offset of 16-byte chunk c of tile row r (kSwz-byte rows, chunk groups
-// of kSwz bytes one after the other).
+// Byte offset of 16-byte chunk c of tile row r (SWZ-byte rows, chunk groups of
+// SWZ bytes one after the other).
 template <int SWZ, int TOK>
 __device__ __forceinline__ uint32_t attend_swz(int r, int c) {
   if (SWZ == 128) return (uint32_t)((c >> 3) * TOK * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -114,11 +128,12 @@ __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t& lo, uint32_t&
   }
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-      : "memory");
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// One arrival on the barrier when this thread's copy16_async calls so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // x0, x1 as TERMS 16-bit pairs whose sum is x to TERMS * 8 (bf16) or 11 bits.
@@ -133,84 +148,92 @@ __device__ __forceinline__ void split_terms(float x0, float x1, uint32_t (&out)[
   }
 }
 
+// A reference below every score (finite, so that differences to -inf stay
+// -inf): the weights of a column that has seen nothing are 2^-inf.
+constexpr float kNoRef = -1e30f;
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// ------------------------------------------------------------------ consumer
 // Columns of a warp: query fragments, accumulators, softmax state.  Lane
-// (g, t) = (lane / 4, lane % 4) holds the query of column g of each n-tile and
-// the accumulators of columns 2t and 2t + 1.
-template <int KV, bool QF32, int D, int NT>
+// (g, t) = (lane / 4, lane % 4) holds the query of column g and the
+// accumulators of columns 2t and 2t + 1.
+template <int KV, bool QF32, int D, int CW>
 struct AttendCols {
-  using G = AttendGeom<KV, QF32, D, NT>;
-  uint32_t q[NT][D / 16][2][G::kQTerms];
-  float acc[NT][D / 16][4];
-  float m[NT][2], l[NT][2], sc[NT][2];  // sc: score scale in base 2
-  int lim[NT][2];
-  int min_lim;  // least limit of the chunk's columns
+  using G = AttendGeom<KV, QF32, D, CW>;
+  uint32_t q[D / 16][2][G::kQTerms];
+  float acc[D / 16][4];
+  float m[2], l[2], sc[2];  // sc: score scale in base 2
+  int lim[2];
+  int min_lim;  // least limit of the warp's columns
 };
 
-template <int KV, bool QF32, int D, int NT>
-__device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& cur, int kvh, int chunk,
-                                             AttendCols<KV, QF32, D, NT>& c, int lane) {
-  using G = AttendGeom<KV, QF32, D, NT>;
+// First of the warp's columns within the (sequence, KV head): chunk * cols + 8 cw.
+template <int KV, bool QF32, int D, int CW>
+__device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& cur, int kvh, int col0,
+                                             AttendCols<KV, QF32, D, CW>& c, int lane) {
+  using G = AttendGeom<KV, QF32, D, CW>;
   using T = typename KvMma<KV>::T;
   constexpr bool kNorm = G::kEight || (KV == KV_F16 && QF32);
   const int half = D / 2;
   const int cap = cur.s.ctx;
-  int least = cap;
+  const AttendCol ci = attend_col(a, cur.s.row0, cur.s.nq, kvh, col0 + (lane >> 2));
+  const int64_t qb = (int64_t)ci.row * a.q_stride + (int64_t)ci.head * D;
+  float x[D / 16][4];
+  uint32_t big = 0;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const AttendCol ci =
-        attend_col(a, cur.s.row0, cur.s.nq, kvh, chunk * (8 * NT) + nt * 8 + (lane >> 2));
-    const int64_t qb = (int64_t)ci.row * a.q_stride + (int64_t)ci.head * D;
-    float x[D / 16][4];
-    uint32_t big = 0;
+  for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = G::kEight ? kk * 16 + (lane & 3) * 4 + i
-                                : kk * 16 + (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
-        const bool in = ci.valid && (a.maps == 1 || (d >= half) == (ci.map == 1));
-        x[kk][i] = in ? attend_load_q(a, qb + d) : 0.f;
-        big = max(big, abs_bits(x[kk][i]));
+    for (int i = 0; i < 4; ++i) {
+      const int d = G::kEight ? kk * 16 + (lane & 3) * 4 + i
+                              : kk * 16 + (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
+      const bool in = ci.valid && (a.maps == 1 || (d >= half) == (ci.map == 1));
+      x[kk][i] = 0.f;
+      if (in) {
+        if (QF32) x[kk][i] = static_cast<const float*>(a.q)[qb + d];
+        else if (a.q_dtype == CLOVER_B200_F16) x[kk][i] = __half2float(static_cast<const __half*>(a.q)[qb + d]);
+        else x[kk][i] = __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[qb + d]);
       }
+      big = max(big, abs_bits(x[kk][i]));
     }
-    float inv = 1.f;
-    if (kNorm) {
-      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      const int e = (int)(big >> 23);
-      const int fe = e == 0 || e == 255 ? 127 : min(268 - e, 253);  // zero, Inf and NaN stay as they are
-      const float f = __uint_as_float((uint32_t)fe << 23);
-      inv = __uint_as_float((uint32_t)(254 - fe) << 23);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[kk][i] *= f;
-    }
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      split_terms<T, G::kQTerms>(x[kk][0], x[kk][1], c.q[nt][kk][0]);
-      split_terms<T, G::kQTerms>(x[kk][2], x[kk][3], c.q[nt][kk][1]);
-    }
-    // limits and score scales of columns 2t, 2t + 1 from the lanes that hold them
-    int lim = ci.valid ? ci.lim : 0;
-    if (lim > cap) {  // a row past its sequence's last row
-      raise_status(a.status, CLOVER_B200_DEV_CTX_RANGE);
-      lim = cap;
-    }
-    if (ci.valid) least = min(least, lim);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int src = ((lane & 3) * 2 + e) * 4;
-      c.lim[nt][e] = __shfl_sync(0xffffffffu, lim, src);
-      c.sc[nt][e] = a.scale_log2 * __shfl_sync(0xffffffffu, inv, src);
-      c.m[nt][e] = -INFINITY;
-      c.l[nt][e] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-      c.acc[nt][i][0] = c.acc[nt][i][1] = c.acc[nt][i][2] = c.acc[nt][i][3] = 0.f;
   }
-  c.min_lim = __reduce_min_sync(0xffffffffu, least);
+  float inv = 1.f;
+  if (kNorm) {
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const int e = (int)(big >> 23);
+    const int fe = e == 0 || e == 255 ? 127 : min(268 - e, 253);  // zero, Inf and NaN stay as they are
+    const float f = __uint_as_float((uint32_t)fe << 23);
+    inv = __uint_as_float((uint32_t)(254 - fe) << 23);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[kk][i] *= f;
+  }
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    split_terms<T, G::kQTerms>(x[kk][0], x[kk][1], c.q[kk][0]);
+    split_terms<T, G::kQTerms>(x[kk][2], x[kk][3], c.q[kk][1]);
+  }
+  // limits and score scales of columns 2t, 2t + 1 from the lanes that hold them
+  int lim = ci.valid ? ci.lim : 0;
+  if (lim > cap) {  // a row past its sequence's last row
+    raise_status(a.status, CLOVER_B200_DEV_CTX_RANGE);
+    lim = cap;
+  }
+  c.min_lim = __reduce_min_sync(0xffffffffu, ci.valid ? lim : cap);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int src = ((lane & 3) * 2 + e) * 4;
+    c.lim[e] = __shfl_sync(0xffffffffu, lim, src);
+    c.sc[e] = a.scale_log2 * __shfl_sync(0xffffffffu, inv, src);
+    c.m[e] = kNoRef;
+    c.l[e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) c.acc[i][0] = c.acc[i][1] = c.acc[i][2] = c.acc[i][3] = 0.f;
 }
 
 // Fragments of V^T, tokens 16 mt .. 16 mt + 15, for dims 16 i .. 16 i + 15 (8
@@ -235,17 +258,21 @@ struct VFrag {
       ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp & 1)), a[0][0], a[0][1], a[0][2], a[0][3]);
     }
   }
+  // Zero the tokens at and past n (of the stage): lo masks tokens 2t, 2t + 1 of
+  // the M tile, hi the tokens 8 later.
+  __device__ __forceinline__ void mask(int mt, int n, int lane) {
+    const int t = mt * 16 + (lane & 3) * 2;
+    const uint32_t lo = (t < n ? 0xffffu : 0u) | (t + 1 < n ? 0xffff0000u : 0u);
+    const uint32_t hi = (t + 8 < n ? 0xffffu : 0u) | (t + 9 < n ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      a[k][0] &= lo;
+      a[k][1] &= lo;
+      a[k][2] &= hi;
+      a[k][3] &= hi;
+    }
+  }
 };
-
-// Zero V rows [r0, TOK) of a stage.
-template <int ROW, int SWZ, int TOK>
-__device__ __forceinline__ void zero_rows(uint8_t* v, int r0, int lane) {
-  constexpr int kC = ROW / 16;
-  for (int i = lane; i < (TOK - r0) * kC; i += 32)
-    *reinterpret_cast<uint4*>(v + attend_swz<SWZ, TOK>(r0 + i / kC, i % kC)) = make_uint4(0, 0, 0, 0);
-  fence_proxy_async_smem();  // before the next copy into this slot
-  __syncwarp();
-}
 
 // Whether rows [r0, r1) of a V tile hold an infinity or NaN (codes: e4m3 NaN).
 template <int KV, int ROW, int SWZ, int TOK>
@@ -270,28 +297,23 @@ __device__ __forceinline__ bool rows_nonfinite(const uint8_t* v, int r0, int r1,
 }
 
 // One stage of one warp.
-template <int KV, bool QF32, int D, int NT>
-__device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, uint8_t* vgen, const float* scales,
-                                             int tok0, int nvalid, AttendCols<KV, QF32, D, NT>& c, int lane) {
-  using G = AttendGeom<KV, QF32, D, NT>;
+template <int KV, bool QF32, int D, int CW>
+__device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, const uint8_t* vgen, const float* scales,
+                                             int tok0, int nvalid, AttendCols<KV, QF32, D, CW>& c, int lane) {
+  using G = AttendGeom<KV, QF32, D, CW>;
   using T = typename KvMma<KV>::T;
   using VF = VFrag<KV, G::kSwz, G::kTok>;
   constexpr int KK = D / 16, QT = G::kQTerms, PT = G::kPTerms, MT = G::kTok / 16;
-  constexpr int CH = MT * NT == 1 ? 2 : 1;  // independent chains per score tile
+  constexpr int CH = 2;  // independent chains per score tile
   const int g = lane >> 2;
 
-  // ---- S = K . Q^T, in base 2 with the scales, masked
-  float s[MT][NT][4];
-  float mx[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+  // ---- S = K . Q^T, times K's scale
+  float s[MT][4];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    float ch[NT][CH][4];
+    float ch[CH][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < CH; ++k) ch[nt][k][0] = ch[nt][k][1] = ch[nt][k][2] = ch[nt][k][3] = 0.f;
+    for (int k = 0; k < CH; ++k) ch[k][0] = ch[k][1] = ch[k][2] = ch[k][3] = 0.f;
     const int r = mt * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
     if (G::kEight) {
 #pragma unroll
@@ -304,10 +326,8 @@ __device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, uint8_t* 
           codes_to_f16<KV, false>(x[2 * k], a0, a2);
           codes_to_f16<KV, false>(x[2 * k + 1], a1, a3);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < QT; ++q)
-              MmaOp<T>::run(ch[nt][k % CH], a0, a1, a2, a3, c.q[nt][2 * i + k][0][q], c.q[nt][2 * i + k][1][q]);
+          for (int q = 0; q < QT; ++q)
+            MmaOp<T>::run(ch[k % CH], a0, a1, a2, a3, c.q[2 * i + k][0][q], c.q[2 * i + k][1][q]);
         }
       }
     } else {
@@ -316,165 +336,241 @@ __device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, uint8_t* 
         uint32_t a0, a1, a2, a3;
         ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, kk * 2 + (lane >> 4)), a0, a1, a2, a3);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int q = 0; q < QT; ++q)
-            MmaOp<T>::run(ch[nt][kk % CH], a0, a1, a2, a3, c.q[nt][kk][0][q], c.q[nt][kk][1][q]);
+        for (int q = 0; q < QT; ++q)
+          MmaOp<T>::run(ch[kk % CH], a0, a1, a2, a3, c.q[kk][0][q], c.q[kk][1][q]);
       }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = mt * 16 + g + 8 * h, t = tok0 + row;
-      float ksc = 1.f, ve = 0.f;
-      if (G::kEight) {
-        ksc = scales[row];
-        // 2^ve >= V's scale; scales below 2^-110 count as that (2^-107 is the least stored)
-        ve = fmaxf((float)((int)(__float_as_uint(scales[G::kTok + row]) >> 23 & 255u) - 126), -110.f);
+      const float ksc = G::kEight ? scales[mt * 16 + g + 8 * h] : 1.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = ch[0][2 * h + e] + ch[1][2 * h + e];
+        s[mt][2 * h + e] = G::kEight ? x * ksc : x;
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float raw = ch[nt][0][2 * h + e];
-          if (CH == 2) raw += ch[nt][CH - 1][2 * h + e];
-          raw *= c.sc[nt][e];
-          const float x = t < c.lim[nt][e] ? (G::kEight ? raw * ksc : raw) : -INFINITY;
-          s[mt][nt][2 * h + e] = x;
-          mx[nt][e] = fmaxf(mx[nt][e], G::kEight ? x + ve : x);
-        }
     }
   }
+  // Stages that every column sees whole need no mask.
+  const bool edge = tok0 + G::kTok > c.min_lim;
+  auto masked = [&](int mt, int h, int e) { return edge && tok0 + mt * 16 + g + 8 * h >= c.lim[e]; };
 
-  // ---- the reference: move it when a column outgrows it
+  // ---- the reference: move it when some weight outgrows it.  Each lane looks
+  // at its own scores; only a move takes the columns' maxima over the lanes.
+  float y[MT][4], ve[MT][2];
   bool moved = false;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int h = 0; h < 2; ++h) {
+      ve[mt][h] = 0.f;
+      // 2^ve >= V's scale; scales below 2^-110 count as that (2^-107 is the least stored)
+      if (G::kEight)
+        ve[mt][h] = fmaxf((float)((int)(__float_as_uint(scales[G::kTok + mt * 16 + g + 8 * h]) >> 23 & 255u) - 126),
+                          -110.f);
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1)
-        mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], off));
-      moved |= mx[nt][e] > c.m[nt][e] + 8.f;
+      for (int e = 0; e < 2; ++e) {
+        y[mt][2 * h + e] = masked(mt, h, e) ? -INFINITY : fmaf(s[mt][2 * h + e], c.sc[e], -c.m[e]);
+        moved |= y[mt][2 * h + e] + ve[mt][h] > 8.f;
+      }
     }
   if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int e = 0; e < 2; ++e) {
+      float mx = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float nm = fmaxf(c.m[nt][e], mx[nt][e]);
-        const float al = fast_exp2(c.m[nt][e] - (nm == -INFINITY ? 0.f : nm));
-        c.m[nt][e] = nm;
-        c.l[nt][e] *= al;
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < KK; ++i) {
-          c.acc[nt][i][e] *= al;
-          c.acc[nt][i][2 + e] *= al;
-        }
+        for (int h = 0; h < 2; ++h)
+          if (!masked(mt, h, e)) mx = fmaxf(mx, fmaf(s[mt][2 * h + e], c.sc[e], ve[mt][h]));
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      const float nm = fmaxf(c.m[e], mx);
+      const float al = fast_exp2(c.m[e] - nm);
+      c.m[e] = nm;
+      c.l[e] *= al;
+#pragma unroll
+      for (int i = 0; i < KK; ++i) {
+        c.acc[i][e] *= al;
+        c.acc[i][2 + e] *= al;
       }
-  }
-
-  // Rows that some column does not see: past the context they are zeroed; a
-  // later token's infinity or NaN must not meet the zero weight of an earlier
-  // row (multi-token rows), so such a stage takes its columns limit by limit,
-  // zeroing rows as it goes.
-  bool plain = true;
-  if (KV != KV_I8 && tok0 + G::kTok > c.min_lim) {
-    if (nvalid < G::kTok) zero_rows<G::kRow, G::kSwz, G::kTok>(vgen, nvalid, lane);
-    const int lo = max(0, c.min_lim - tok0), hi = min(nvalid, G::kTok);
-    if (lo < hi && rows_nonfinite<KV, G::kRow, G::kSwz, G::kTok>(vgen, lo, hi, lane)) plain = false;
-  }
-
-  // ---- weights, split and transposed; O^T += V^T . P^T
-  uint32_t pt[MT][NT][2][PT];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          y[mt][2 * h + e] = masked(mt, h, e) ? -INFINITY : fmaf(s[mt][2 * h + e], c.sc[e], -nm);
+    }
+  }
+
+  // ---- weights, split and transposed
+  uint32_t pt[MT][2][PT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = mt * 16 + g + 8 * h, t = tok0 + row;
-      const float vsc = G::kEight ? scales[G::kTok + row] : 1.f;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float p0 = fast_exp2(s[mt][nt][2 * h] - (c.m[nt][0] == -INFINITY ? 0.f : c.m[nt][0]));
-        float p1 = fast_exp2(s[mt][nt][2 * h + 1] - (c.m[nt][1] == -INFINITY ? 0.f : c.m[nt][1]));
-        c.l[nt][0] += p0;
-        c.l[nt][1] += p1;
-        if (G::kEight) {  // (a masked token's scale may be anything)
-          p0 = t < c.lim[nt][0] ? p0 * vsc : 0.f;
-          p1 = t < c.lim[nt][1] ? p1 * vsc : 0.f;
-        }
-        split_terms<T, PT>(p0, p1, pt[mt][nt][h]);
-#pragma unroll
-        for (int k = 0; k < PT; ++k) pt[mt][nt][h][k] = movm_trans(pt[mt][nt][h][k]);
+      float p0 = fast_exp2(y[mt][2 * h]), p1 = fast_exp2(y[mt][2 * h + 1]);
+      c.l[0] += p0;
+      c.l[1] += p1;
+      if (G::kEight) {  // (a masked token's scale may be anything: its weight stays 0)
+        const float vsc = scales[G::kTok + mt * 16 + g + 8 * h];
+        p0 = edge && p0 == 0.f ? 0.f : p0 * vsc;
+        p1 = edge && p1 == 0.f ? 0.f : p1 * vsc;
       }
+      split_terms<T, PT>(p0, p1, pt[mt][h]);
+#pragma unroll
+      for (int k = 0; k < PT; ++k) pt[mt][h][k] = movm_trans(pt[mt][h][k]);
     }
-    if (plain) {
-#pragma unroll
-      for (int i = 0; i < KK / VF::kPer; ++i) {
-        VF v;
-        v.load(vs, mt, i, lane);
-#pragma unroll
-        for (int k = 0; k < VF::kPer; ++k)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < PT; ++q)
-              MmaOp<T>::run(c.acc[nt][i * VF::kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3],
-                            pt[mt][nt][0][q], pt[mt][nt][1][q]);
-      }
-    }
-  }
-  if (plain) return;
-  for (int below = 0x7fffffff;;) {
-    int top = 0;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (c.lim[nt][e] < below) top = max(top, c.lim[nt][e]);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (top <= tok0) break;
-    if (top - tok0 < G::kTok) zero_rows<G::kRow, G::kSwz, G::kTok>(vgen, top - tok0, lane);
+
+  // ---- O^T += V^T . P^T
+  if (KV == KV_I8 || !edge) {  // (every int8 code is finite)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < KK / VF::kPer; ++i) {
         VF v;
         v.load(vs, mt, i, lane);
 #pragma unroll
         for (int k = 0; k < VF::kPer; ++k)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < PT; ++q)
-              MmaOp<T>::run(x, v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[mt][nt][0][q], pt[mt][nt][1][q]);
-            // (constant indices: the accumulators stay in registers)
-#pragma unroll
-            for (int j = 0; j < KK; ++j) {
-              if (j != i * VF::kPer + k) continue;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (c.lim[nt][e & 1] == top) c.acc[nt][j][e] += x[e];
-            }
-          }
+          for (int q = 0; q < PT; ++q)
+            MmaOp<T>::run(c.acc[i * VF::kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[mt][0][q],
+                          pt[mt][1][q]);
       }
+    return;
+  }
+  // Tokens that some column does not see.  Past the context they are masked in
+  // V; an infinity or NaN of a later token must not meet the zero weight of an
+  // earlier row (multi-token rows), so a stage that holds one takes its columns
+  // limit by limit, each with V masked from its limit on.
+  const int lo = max(0, c.min_lim - tok0), hi = min(nvalid, G::kTok);
+  const bool plain = !(lo < hi && rows_nonfinite<KV, G::kRow, G::kSwz, G::kTok>(vgen, lo, hi, lane));
+  for (int below = 0x7fffffff;;) {
+    int top = plain ? tok0 + hi : 0;
+    if (!plain) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (c.lim[e] < below) top = max(top, c.lim[e]);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (top <= tok0) break;
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < KK / VF::kPer; ++i) {
+        VF v;
+        v.load(vs, mt, i, lane);
+        v.mask(mt, top - tok0, lane);
+#pragma unroll
+        for (int k = 0; k < VF::kPer; ++k) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < PT; ++q)
+            MmaOp<T>::run(x, v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[mt][0][q], pt[mt][1][q]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (plain || c.lim[e & 1] == top) c.acc[i * VF::kPer + k][e] += x[e];
+        }
+      }
+    if (plain) break;
     below = top;
   }
 }
 
-// Fused append: the new tokens of the cursor's sequence that lie in its unit,
-// for KV head kvh, written before the unit is copied (slot[u]: first cache slot
-// of the unit's u-th 16 tokens).
+// The end of a segment's piece: the output, or a partial for the join.
+template <int KV, bool QF32, int D, int CW>
+__device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& cur, int wid, const AttendSplit& sp,
+                                             int first_jj, int kvh, int chunk, int cw,
+                                             AttendCols<KV, QF32, D, CW>& c, int lane) {
+  using G = AttendGeom<KV, QF32, D, CW>;
+  constexpr int KK = D / 16, COLS = 8 * CW;
+  const bool whole = a.whole || (first_jj == 0 && cur.jj == cur.s.n - 1);
+#pragma unroll
+  for (int off = 4; off < 32; off <<= 1) {
+    c.l[0] += __shfl_xor_sync(0xffffffffu, c.l[0], off);
+    c.l[1] += __shfl_xor_sync(0xffffffffu, c.l[1], off);
+  }
+  const int g = lane >> 2, c0 = cw * 8 + (lane & 3) * 2;
+  const int d0 = G::kEight ? 2 * g : g, dh = G::kEight ? 1 : 8;  // dims of M rows g, g + 8
+  if (!whole) {
+    const int64_t slot = attend_slot(sp, wid, first_jj);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t at = slot * COLS + c0 + e;
+      float* po = a.part + at * D;
+#pragma unroll
+      for (int i = 0; i < KK; ++i) {
+        if (G::kEight) {
+          *reinterpret_cast<float2*>(po + i * 16 + d0) = make_float2(c.acc[i][e], c.acc[i][2 + e]);
+        } else {
+          po[i * 16 + d0] = c.acc[i][e];
+          po[i * 16 + d0 + dh] = c.acc[i][2 + e];
+        }
+      }
+      if (lane < 4) a.part_ml[at] = make_float2(c.m[e], c.l[e]);
+    }
+  } else if (a.maps == 1) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const AttendCol ci = attend_col(a, cur.s.row0, cur.s.nq, kvh, chunk * COLS + c0 + e);
+      if (!ci.valid) continue;
+      const bool any = c.lim[e] > 0;
+      const float inv = attend_inv(c.l[e], c.lim[e]);
+      const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D + d0;
+#pragma unroll
+      for (int i = 0; i < KK; ++i) {
+        attend_store(a, ob + i * 16, any ? c.acc[i][e] * inv : 0.f);
+        attend_store(a, ob + i * 16 + dh, any ? c.acc[i][2 + e] * inv : 0.f);
+      }
+    }
+  } else {
+    // columns 2t and 2t + 1 are the two maps of one head
+    const AttendCol ci = attend_col(a, cur.s.row0, cur.s.nq, kvh, chunk * COLS + c0);
+    const bool any = c.lim[0] > 0;
+    const float lam = ci.valid ? a.lam[ci.head] : 0.f;
+    const float i0 = attend_inv(c.l[0], c.lim[0]), i1 = attend_inv(c.l[1], c.lim[1]);
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < KK; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float o = any ? diff_value(c.acc[i][2 * h] * i0, c.acc[i][2 * h + 1] * i1, lam) : 0.f;
+        c.acc[i][2 * h] = o;
+        sq = fmaf(o, o, sq);
+      }
+    }
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
+    if (ci.valid) {
+      const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D;
+      const float r = a.norm_w != nullptr ? rsqrtf(sq / D + a.eps) * a.out_scale : 1.f;
+#pragma unroll
+      for (int i = 0; i < KK; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = i * 16 + d0 + h * dh;
+          const float w = a.norm_w != nullptr ? a.norm_w[d] : 1.f;
+          attend_store(a, ob + d, c.acc[i][2 * h] * (r * w));
+        }
+      }
+    }
+    __syncwarp();
+  }
+  if (!a.whole && first_jj == 0 && cw == 0 && lane == 0)
+    attend_record(a, sp, cur.b, cur.h, cur.seg0, cur.s, wid);
+}
+
+// ------------------------------------------------------------------ copies
+// Fused append: the new tokens of a sequence (rows row0 .. row0 + nq - 1) that
+// lie in the unit [tok0, tok0 + 16 SUBS), for KV head kvh, written by the warp
+// before the unit is copied (slot0, slot1: first cache slot of its 16-token
+// steps).
 template <int KV, int D, int SUBS>
-__device__ __forceinline__ void append_unit(const AttendArgs& a, const Cursor& cur, int kvh,
-                                            const int (&slot)[SUBS], int lane) {
-  const int tok0 = cur.jj * SUBS * kUnitTok;
-  for (int j = 0; j < cur.s.nq; ++j) {
-    const int r = cur.s.row0 + j;
+__device__ __forceinline__ void append_unit(const AttendArgs& a, int row0, int nq, int ctx, int tok0, int kvh,
+                                            int slot0, int slot1, int lane) {
+  for (int j = 0; j < nq; ++j) {
+    const int r = row0 + j;
     const int rel = __ldg(a.ctx + r) - 1 - tok0;
-    if (rel < 0 || rel >= SUBS * kUnitTok || rel + tok0 >= cur.s.ctx) continue;
-    const int base = SUBS == 1 || rel < kUnitTok ? slot[0] : slot[SUBS - 1];
-    const int64_t at = base + (rel & (kUnitTok - 1));
+    if (rel < 0 || rel >= SUBS * kUnitTok || rel + tok0 >= ctx) continue;
+    const int64_t at = (rel < kUnitTok ? slot0 : slot1) + (rel & (kUnitTok - 1));
     const int64_t row = (at * a.hkv + kvh) * D, src = (int64_t)r * a.new_stride + (int64_t)kvh * D;
     if (KV >= KV_I8) {
       uint8_t* kd = static_cast<uint8_t*>(const_cast<void*>(a.kc)) + row;
@@ -499,21 +595,107 @@ __device__ __forceinline__ void append_unit(const AttendArgs& a, const Cursor& c
   __syncwarp();
 }
 
-template <int KV, bool QF32, int D, int NT>
-__global__ void __launch_bounds__(kAttendThreads, AttendGeom<KV, QF32, D, NT>::kCtas)
+// The copies of a ring: the unit after the last one issued, and where its
+// tokens are.  Block ids are held 32 at a time (lane i: block id_base + i).
+template <int KV, bool QF32, int D, int CW>
+struct RingCopies {
+  using G = AttendGeom<KV, QF32, D, CW>;
+  Cursor cur;
+  bool more;
+  int ids, id_base, blk, sub, kvh, first_new, st;
+
+  // Start (or go on in) a segment: the block and 16-token step of its unit jj.
+  __device__ __forceinline__ void enter(const AttendArgs& a, bool new_seq) {
+    const int upb = a.bs / kUnitTok;
+    if (new_seq) id_base = -64;
+    kvh = cur.h / (cur.s.hc / a.hkv);
+    const int at = cur.jj * G::kSubs;
+    blk = at / upb;
+    sub = at - blk * upb;
+    if (a.k_new != nullptr) first_new = __ldg(a.ctx + cur.s.row0) - 1;
+  }
+
+  __device__ __forceinline__ void issue(const AttendArgs& a, const CUtensorMap* tmK, const CUtensorMap* tmV,
+                                        uint32_t ring, uint32_t scales, uint32_t full, int lane) {
+    constexpr int SUBS = G::kSubs;
+    const int upb = a.bs / kUnitTok;
+    if (blk < id_base || blk + SUBS > id_base + 32) {
+      id_base = blk;
+      const int trow = a.seq_rows ? __ldg(a.seq_rows + cur.b) : cur.b;
+      const int n = (cur.s.ctx + a.bs - 1) / a.bs;
+      ids = 0;
+      if (blk + lane < n) {
+        ids = blk + lane < a.table_stride ? __ldg(a.tables + (int64_t)trow * a.table_stride + blk + lane) : -1;
+        if (ids < 0 || ids >= a.num_blocks) {
+          raise_status(a.status, CLOVER_B200_DEV_BAD_BLOCK);
+          ids = 0;  // keep the pipeline well-formed; the output is flagged
+        }
+      }
+    }
+    int slot[SUBS];  // first cache slot of each 16-token step
+    int id[SUBS], off[SUBS];
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      id[u] = __shfl_sync(0xffffffffu, ids, blk - id_base);
+      off[u] = sub * kUnitTok;
+      slot[u] = id[u] * a.bs + off[u];
+      if (++sub == upb) {
+        sub = 0;
+        ++blk;
+      }
+    }
+    if (a.k_new != nullptr && (cur.jj + 1) * G::kTok > first_new)
+      append_unit<KV, D, SUBS>(a, cur.s.row0, cur.s.nq, cur.s.ctx, cur.jj * G::kTok, kvh, slot[0], slot[SUBS - 1],
+                               lane);
+    const int left = (cur.s.ctx + kUnitTok - 1) / kUnitTok - cur.jj * SUBS;  // steps of the segment
+    const int subs = left < SUBS ? left : SUBS;
+    const uint32_t bar = full + st * 8;
+    const uint32_t kd = ring + st * G::kTiles, vd = kd + G::kTile;
+    if (lane == 0) mbar_arrive_expect_tx(bar, subs * (G::kTiles / SUBS));
+    __syncwarp();
+    // one tile copy per lane: (step, chunk, K or V)
+    constexpr int kPer = 2 * G::kChunks;
+    const int u = lane / kPer, i = lane - u * kPer;
+    if (u < subs) {
+      const int ch = i >> 1;
+      tma_load_3d((i & 1 ? vd : kd) + (ch * G::kTok + u * kUnitTok) * G::kSwz, i & 1 ? tmV : tmK,
+                  ch * (G::kSwz / G::kEsz), kvh, u == 0 ? slot[0] : slot[SUBS - 1], bar);
+    }
+    if (G::kEight) {
+      // 16 bytes of the scales per lane: (K or V, step, quarter)
+      const int su = SUBS > 1 ? (lane >> 2) & 1 : 0, v = SUBS > 1 ? lane >> 3 : lane >> 2;
+      if (v < 2 && su < subs) {
+        const int64_t at = ((int64_t)(su ? id[SUBS - 1] : id[0]) * a.hkv + kvh) * a.bs + (su ? off[SUBS - 1] : off[0]);
+        copy16_async(scales + st * G::kScales + (v * G::kTok + su * kUnitTok) * 4 + (lane & 3) * 16,
+                     (v ? a.vs : a.ks) + at + (lane & 3) * 4);
+      }
+      copies_arrive(bar);
+    }
+    st = st + 1 == G::kStages ? 0 : st + 1;
+    const int b = cur.b, h = cur.h;
+    more = cur.next(a);
+    if (more && (cur.b != b || cur.h != h)) enter(a, cur.b != b);
+  }
+};
+
+template <int KV, bool QF32, int D, int CW>
+__global__ void __launch_bounds__(AttendGeom<KV, QF32, D, CW>::kThreads, 1)
 attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const AttendArgs a) {
-  using G = AttendGeom<KV, QF32, D, NT>;
-  constexpr int STAGES = G::kStages;
-  constexpr int KK = D / 16;
+  using G = AttendGeom<KV, QF32, D, CW>;
+  constexpr int STAGES = G::kStages, RINGS = G::kRings, COLS = 8 * CW;
+  constexpr int LAG = CW > 1 ? 1 : 0;  // a shared stage is refilled one unit later
+  static_assert(STAGES > LAG, "a refill may not wait for itself");
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[kAttendWarps * STAGES];
-  __shared__ AttendPlan plan;
+  __shared__ __align__(8) uint64_t s_full[RINGS * STAGES], s_empty[RINGS * STAGES];
+  __shared__ AttendPlan<G::kWarps, RINGS> plan;
   __shared__ int s_stop;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int wid = blockIdx.x * kAttendWarps + warp;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kAttendWarps * STAGES; ++i) mbar_init(smem_addr(&bars[i]), 1);
+    for (int i = 0; i < RINGS * STAGES; ++i) {
+      mbar_init(smem_addr(&s_full[i]), G::kEight ? 33 : 1);  // the tiles, and each lane's scales
+      mbar_init(smem_addr(&s_empty[i]), 1);                  // the ring's other warp
+    }
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -525,251 +707,108 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __syncthreads();
   if (s_stop) return;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + warp * G::kWarpTiles;
-  float* scales = reinterpret_cast<float*>(smem + kAttendWarps * G::kWarpTiles) + warp * STAGES * (G::kScales / 4);
-  const uint32_t ring_s = smem_addr(ring), scales_s = smem_addr(scales), bar0 = smem_addr(&bars[warp * STAGES]);
-  const int hcmax = a.hkv * a.chunks;
+  uint8_t* smem_sc = smem + RINGS * G::kRingTiles;
+  AttendSplit sp{1, 0, false};
+  if (!a.whole) {
+    sp = attend_plan<G::kWarps, RINGS>(a, plan);
+    pdl_trigger();
+  }
 
-  int per = 1;
-  Cursor pc;  // the copies' position
-  bool more;
-  if (a.whole) {
+  // ring r of this CTA is worker r * gridDim.x + blockIdx.x: few workers spread
+  // over the SMs
+  const int ring = warp / CW, cw = warp % CW;
+  const int wid = ring * gridDim.x + blockIdx.x;
+  if (a.whole && cw == 0) {
     // rows of empty sequences have no unit: their zeros are written here
+    const int hcmax = a.hkv * a.chunks;
     for (int64_t sg = wid; sg < (int64_t)a.n_seqs * hcmax; sg += a.workers) {
       const int b = (int)sg / hcmax, h = (int)sg - b * hcmax;
       const SeqInfo s = seq_info(a, b);
       if (h == 0 && lane == 0) attend_check_seq(a, s);
       if (h >= s.hc || s.n > 0) continue;
       const int nch = s.hc / a.hkv, kvh = h / nch;
-      for (int c = 0; c < 8 * NT; ++c) {
-        const AttendCol ci = attend_col(a, s.row0, s.nq, kvh, (h - kvh * nch) * (8 * NT) + c);
+      for (int c = 0; c < COLS; ++c) {
+        const AttendCol ci = attend_col(a, s.row0, s.nq, kvh, (h - kvh * nch) * COLS + c);
         if (!ci.valid || ci.map == 1) continue;
         for (int d = lane; d < D; d += 32)
           attend_store(a, (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D + d, 0.f);
       }
     }
-    more = pc.seek(a, wid);
-  } else {
-    int total;
-    per = attend_plan(a, plan, total);
-    pdl_trigger();
-    const int64_t u0 = (int64_t)wid * per;
-    more = u0 < total && plan.start[warp][0] >= 0;
-    if (more)
-      pc.start(a, plan.start[warp][0], plan.start[warp][1], plan.start[warp][2],
-               (int)min((int64_t)per, total - u0));
   }
-  if (!more) return;
-  Cursor cc = pc;  // the products' position
+  Cursor cur;
+  if (!(a.whole ? cur.seek(a, wid) : attend_start(a, plan, ring, cur))) return;
+  const uint32_t ring_s = smem_addr(smem) + ring * G::kRingTiles;
+  const uint32_t scales_s = smem_addr(smem_sc) + ring * STAGES * G::kScales;
+  const uint32_t full = smem_addr(&s_full[ring * STAGES]), empty = smem_addr(&s_empty[ring * STAGES]);
 
-  // ---- copies.  Block ids of the sequence are held 32 at a time (lane i:
-  // block id_base + i); block and sub count 16-token steps of the segment.
-  constexpr int SUBS = G::kTok / kUnitTok;
-  const int upb = a.bs / kUnitTok;  // 16-token steps per block
-  int ids = 0, id_base = -64, p_b = -1, p_h = -1, p_kvh = 0, blk_i = 0, sub = 0, first_new = 0;
-  int p_st = 0;
-  auto issue = [&]() {
-    if (pc.b != p_b || pc.h != p_h) {
-      if (pc.b != p_b) id_base = -64;
-      p_b = pc.b;
-      p_h = pc.h;
-      p_kvh = pc.h / (pc.s.hc / a.hkv);
-      const int at = pc.jj * SUBS;
-      blk_i = at / upb;
-      sub = at - blk_i * upb;
-      if (a.k_new != nullptr) first_new = __ldg(a.ctx + pc.s.row0) - 1;
-    }
-    const int n_sub = (pc.s.ctx + kUnitTok - 1) / kUnitTok - pc.jj * SUBS;  // steps left
-    if (blk_i < id_base || blk_i + SUBS > id_base + 32) {
-      id_base = blk_i;
-      const int trow = a.seq_rows ? __ldg(a.seq_rows + pc.b) : pc.b;
-      const int nblk = (pc.s.ctx + a.bs - 1) / a.bs;
-      ids = 0;
-      if (blk_i + lane < nblk) {
-        ids = blk_i + lane < a.table_stride
-                  ? __ldg(a.tables + (int64_t)trow * a.table_stride + blk_i + lane) : -1;
-        if (ids < 0 || ids >= a.num_blocks) {
-          raise_status(a.status, CLOVER_B200_DEV_BAD_BLOCK);
-          ids = 0;  // keep the pipeline well-formed; the output is flagged
-        }
-      }
-    }
-    int slot[SUBS];  // first cache slot of each 16-token step
-    int64_t sc_at[SUBS];
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
-      const int blk = __shfl_sync(0xffffffffu, ids, blk_i - id_base);
-      slot[u] = blk * a.bs + sub * kUnitTok;
-      sc_at[u] = ((int64_t)blk * a.hkv + p_kvh) * a.bs + sub * kUnitTok;
-      if (++sub == upb) {
-        sub = 0;
-        ++blk_i;
-      }
-    }
-    if (a.k_new != nullptr && (pc.jj + 1) * G::kTok > first_new)
-      append_unit<KV, D>(a, pc, p_kvh, slot, lane);
-    const int subs = n_sub < SUBS ? n_sub : SUBS;
-    const uint32_t bar = bar0 + p_st * 8;
-    const uint32_t kd = ring_s + p_st * G::kTiles, vd = kd + G::kTile;
-    if (lane == 0) mbar_arrive_expect_tx(bar, subs * (G::kStageB / SUBS));
-    __syncwarp();
-    // one copy per lane: (step, K or V, chunk), then the scales
-    constexpr int kCopies = 2 * G::kChunks;
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
-      if (u >= subs) break;
-      const int i = lane - u * (kCopies + 2);
-      if (i >= 0 && i < kCopies) {
-        const int ch = i >> 1;
-        tma_load_3d((i & 1 ? vd : kd) + (ch * G::kTok + u * kUnitTok) * G::kSwz, i & 1 ? &tmV : &tmK,
-                    ch * (G::kSwz / G::kEsz), p_kvh, slot[u], bar);
-      }
-      if (G::kEight && (i == kCopies || i == kCopies + 1)) {
-        const int v = i - kCopies;
-        bulk_load(scales_s + p_st * G::kScales + (v * G::kTok + u * kUnitTok) * 4, (v ? a.vs : a.ks) + sc_at[u],
-                  kUnitTok * 4, bar);
-      }
-    }
-    p_st = p_st + 1 == STAGES ? 0 : p_st + 1;
-  };
-
+  RingCopies<KV, QF32, D, CW> copies;
+  copies.cur = cur;
+  copies.more = cw == 0;
+  copies.st = 0;
+  copies.first_new = 0x7fffffff;
   int issued = 0;
-  while (issued < STAGES && more) {
-    issue();
-    ++issued;
-    more = pc.next(a);
+  if (cw == 0) {
+    copies.enter(a, true);
+    while (issued < STAGES && copies.more) {
+      copies.issue(a, &tmK, &tmV, ring_s, scales_s, full, lane);
+      ++issued;
+    }
   }
 
-  AttendCols<KV, QF32, D, NT> c;
-  int cur_b = -1, cur_h = -1, first_jj = 0, last_jj = 0, kvh = 0, chunk = 0;
-  Cursor seg = cc;  // the segment of the columns in registers
-
-  auto finish = [&]() {
-    const bool whole = a.whole || (first_jj == 0 && last_jj == seg.s.n - 1);
-    const int64_t slot = 2 * (int64_t)wid + (first_jj == 0 ? 1 : 0);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        c.l[nt][0] += __shfl_xor_sync(0xffffffffu, c.l[nt][0], off);
-        c.l[nt][1] += __shfl_xor_sync(0xffffffffu, c.l[nt][1], off);
-      }
-      const int g = lane >> 2, c0 = nt * 8 + (lane & 3) * 2;
-      const int d0 = G::kEight ? 2 * g : g, dh = G::kEight ? 1 : 8;  // dims of M rows g, g + 8
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int64_t at = slot * (8 * NT) + c0 + e;
-          float* po = a.part + at * D;
-#pragma unroll
-          for (int i = 0; i < KK; ++i) {
-            if (G::kEight) {
-              *reinterpret_cast<float2*>(po + i * 16 + d0) = make_float2(c.acc[nt][i][e], c.acc[nt][i][2 + e]);
-            } else {
-              po[i * 16 + d0] = c.acc[nt][i][e];
-              po[i * 16 + d0 + dh] = c.acc[nt][i][2 + e];
-            }
-          }
-          if (lane < 4) a.part_ml[at] = make_float2(c.m[nt][e], c.l[nt][e]);
-        }
-        continue;
-      }
-      if (a.maps == 1) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const AttendCol ci = attend_col(a, seg.s.row0, seg.s.nq, kvh, chunk * (8 * NT) + c0 + e);
-          if (!ci.valid) continue;
-          const bool any = c.lim[nt][e] > 0;
-          const float inv = attend_inv(c.l[nt][e], c.lim[nt][e]);
-          const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D + d0;
-#pragma unroll
-          for (int i = 0; i < KK; ++i) {
-            attend_store(a, ob + i * 16, any ? c.acc[nt][i][e] * inv : 0.f);
-            attend_store(a, ob + i * 16 + dh, any ? c.acc[nt][i][2 + e] * inv : 0.f);
-          }
-        }
-      } else {
-        // columns 2t and 2t + 1 are the two maps of one head
-        const AttendCol ci = attend_col(a, seg.s.row0, seg.s.nq, kvh, chunk * (8 * NT) + c0);
-        const bool any = c.lim[nt][0] > 0;
-        const float lam = ci.valid ? a.lam[ci.head] : 0.f;
-        const float i0 = attend_inv(c.l[nt][0], c.lim[nt][0]), i1 = attend_inv(c.l[nt][1], c.lim[nt][1]);
-        float sq = 0.f;
-#pragma unroll
-        for (int i = 0; i < KK; ++i) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float o = any ? diff_value(c.acc[nt][i][2 * h] * i0, c.acc[nt][i][2 * h + 1] * i1, lam) : 0.f;
-            c.acc[nt][i][2 * h] = o;
-            sq = fmaf(o, o, sq);
-          }
-        }
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-        if (!ci.valid) continue;
-        const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D;
-        const float r = a.norm_w != nullptr ? rsqrtf(sq / D + a.eps) * a.out_scale : 1.f;
-#pragma unroll
-        for (int i = 0; i < KK; ++i) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int d = i * 16 + d0 + h * dh;
-            const float w = a.norm_w != nullptr ? a.norm_w[d] : 1.f;
-            attend_store(a, ob + d, c.acc[nt][i][2 * h] * (r * w));
-          }
-        }
-      }
-    }
-    if (!a.whole && first_jj == 0 && lane == 0) {
-      const int fw = seg.seg0 / per;
-      a.seg[(int64_t)seg.b * hcmax + seg.h] = make_int2(fw, (seg.seg0 + seg.s.n - 1) / per - fw + 1);
-    }
-  };
-
-  bool timed_out = false;
-  int k = 0, st = 0;
+  AttendCols<KV, QF32, D, CW> c;
+  int first_jj = 0, kvh = 0, chunk = 0, st = 0, k = 0;
   uint32_t parity = 0;
+  bool fresh = true, cols = false, timed_out = false;
   for (;; ++k) {
-    if (cc.b != cur_b || cc.h != cur_h) {
-      if (cur_b >= 0) finish();
-      cur_b = cc.b;
-      cur_h = cc.h;
-      seg = cc;
-      first_jj = cc.jj;
-      const int nch = cc.s.hc / a.hkv;
-      kvh = cc.h / nch;
-      chunk = cc.h - kvh * nch;
-      load_columns<KV, QF32, D, NT>(a, cc, kvh, chunk, c, lane);
+    if (fresh) {
+      first_jj = cur.jj;
+      const int nch = cur.s.hc / a.hkv;
+      kvh = cur.h / nch;
+      chunk = cur.h - kvh * nch;
+      // (a column warp past the sequence's columns only passes the stages on)
+      cols = chunk * COLS + cw * 8 < cur.s.nq * a.group * a.maps;
+      if (cols) load_columns<KV, QF32, D, CW>(a, cur, kvh, chunk * COLS + cw * 8, c, lane);
     }
-    if (!mbar_wait_bounded(bar0 + st * 8, parity, a.wait_ns)) {
+    if (!mbar_wait_bounded(full + st * 8, parity, a.wait_ns)) {
       timed_out = true;
       break;
     }
-    last_jj = cc.jj;
-    const int tok0 = cc.jj * G::kTok;
-    const uint32_t ks = ring_s + st * G::kTiles;
-    attend_stage<KV, QF32, D, NT>(ks, ks + G::kTile, ring + st * G::kTiles + G::kTile,
-                                  scales + st * (G::kScales / 4), tok0, cc.s.ctx - tok0, c, lane);
+    if (cols) {
+      const uint32_t ks = ring_s + st * G::kTiles;
+      const int tok0 = cur.jj * G::kTok;
+      attend_stage<KV, QF32, D, CW>(
+          ks, ks + G::kTile, smem + ring * G::kRingTiles + st * G::kTiles + G::kTile,
+          reinterpret_cast<const float*>(smem_sc + (ring * STAGES + st) * G::kScales), tok0, cur.s.ctx - tok0, c,
+          lane);
+    }
     __syncwarp();
-    if (more) {
-      issue();
+    if (CW > 1 && cw > 0 && lane == 0) mbar_arrive(empty + st * 8);
+    if (copies.more && k >= LAG) {
+      // (the stage refilled is copies.st: unit k - LAG was in it)
+      if (CW > 1 && !mbar_wait_bounded(empty + copies.st * 8, ((k - LAG) / STAGES) & 1, a.wait_ns)) {
+        timed_out = true;
+        break;
+      }
+      copies.issue(a, &tmK, &tmV, ring_s, scales_s, full, lane);
       ++issued;
-      more = pc.next(a);
     }
     if (++st == STAGES) {
       st = 0;
       parity ^= 1;
     }
-    if (!cc.next(a)) break;
+    Cursor nx = cur;
+    const bool on = nx.next(a);
+    fresh = !on || nx.b != cur.b || nx.h != cur.h;
+    if (fresh && cols) finish_piece<KV, QF32, D, CW>(a, cur, wid, sp, first_jj, kvh, chunk, cw, c, lane);
+    if (!on) break;
+    cur = nx;
   }
   if (timed_out) {
-    // drain this warp's copies still in flight (bounded) before giving up
-    for (int j = k; j < issued; ++j)
-      mbar_wait_bounded(bar0 + (j % STAGES) * 8, (j / STAGES) & 1, kWaitLimitNs);
+    // the copies in flight land (bounded) before the CTA's memory goes
+    for (int j = max(0, issued - STAGES); j < issued; ++j)
+      mbar_wait_bounded(full + (j % STAGES) * 8, (j / STAGES) & 1, kWaitLimitNs);
     if (lane == 0) raise_status(a.status, CLOVER_B200_DEV_TIMEOUT);
-    return;
   }
-  finish();
 }
 
 // ------------------------------------------------------------------ host side
@@ -825,33 +864,29 @@ static int attend_tmap(const void* ptr, int esz, int D, int H, int64_t slots, CU
   return CLOVER_B200_OK;
 }
 
-template <int KV, bool QF32, int D, int NT>
-static int mma_launch(const AttendArgs* a, cudaStream_t s, int* grid) {
-  using G = AttendGeom<KV, QF32, D, NT>;
-  auto kern = attend_mma_kernel<KV, QF32, D, NT>;
-  static int per_sm[64] = {0}, sms[64] = {0};
+template <int KV, bool QF32, int D, int CW>
+static int mma_launch(const AttendArgs* a, cudaStream_t s, int* grid, int* rings) {
+  using G = AttendGeom<KV, QF32, D, CW>;
+  auto kern = attend_mma_kernel<KV, QF32, D, CW>;
+  static int sms[64] = {0};
   int dev = 0;
   int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   if (rc) return rc;
   if (dev >= 64) return set_error(CLOVER_B200_ERR_UNSUPPORTED, "attend: device ordinal %d", dev);
   {
     std::lock_guard<std::mutex> lock(g_attend_mu);
-    if (per_sm[dev] == 0) {
+    if (sms[dev] == 0) {
       rc = set_smem(kern, G::kSmem);
       if (rc) return rc;
-      int n = 0, m = 0;
-      rc = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kAttendThreads, G::kSmem),
-                      "attend occupancy");
-      if (rc) return rc;
+      int m = 0;
       rc = check_cuda(cudaDeviceGetAttribute(&m, cudaDevAttrMultiProcessorCount, dev), "attend SMs");
       if (rc) return rc;
-      if (n < 1) return set_error(CLOVER_B200_ERR_UNSUPPORTED, "attend: kernel does not fit on an SM");
       sms[dev] = m;
-      per_sm[dev] = n;
     }
   }
   if (a == nullptr) {
-    *grid = per_sm[dev] * sms[dev];
+    *grid = sms[dev];
+    *rings = G::kRings;
     return CLOVER_B200_OK;
   }
   CUtensorMap tk, tv;
@@ -859,17 +894,17 @@ static int mma_launch(const AttendArgs* a, cudaStream_t s, int* grid) {
   if (rc) return rc;
   rc = attend_tmap(a->vc, G::kEsz, D, a->hkv, a->num_blocks * a->bs, &tv);
   if (rc) return rc;
-  return check_cuda(launch_pdl(kern, dim3(a->workers / kAttendWarps), dim3(kAttendThreads), G::kSmem, s, tk, tv, *a),
+  return check_cuda(launch_pdl(kern, dim3(a->workers / G::kRings), dim3(G::kThreads), G::kSmem, s, tk, tv, *a),
                     "attend_mma launch");
 }
 
 template <int KV, bool QF32>
-static int mma_shape(int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid) {
+static int mma_shape(int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid, int* rings) {
   const bool two = cols > kMmaCols;
   switch (D) {
-    case 64: return two ? mma_launch<KV, QF32, 64, 2>(a, s, grid) : mma_launch<KV, QF32, 64, 1>(a, s, grid);
-    case 128: return two ? mma_launch<KV, QF32, 128, 2>(a, s, grid) : mma_launch<KV, QF32, 128, 1>(a, s, grid);
-    default: return mma_launch<KV, QF32, 256, 1>(a, s, grid);
+    case 64: return two ? mma_launch<KV, QF32, 64, 2>(a, s, grid, rings) : mma_launch<KV, QF32, 64, 1>(a, s, grid, rings);
+    case 128: return two ? mma_launch<KV, QF32, 128, 2>(a, s, grid, rings) : mma_launch<KV, QF32, 128, 1>(a, s, grid, rings);
+    default: return two ? mma_launch<KV, QF32, 256, 2>(a, s, grid, rings) : mma_launch<KV, QF32, 256, 1>(a, s, grid, rings);
   }
 }
 
@@ -882,13 +917,13 @@ int attend_mma_unit_log2(int kv_dtype, int D) {
   return D * (eight ? 1 : 2) <= 128 ? 5 : 4;
 }
 
-int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid) {
+int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid, int* rings) {
   const bool f32 = q_dtype == CLOVER_B200_F32;
   switch (kv_dtype) {
-    case CLOVER_B200_BF16: return f32 ? mma_shape<KV_BF16, true>(cols, a, D, s, grid) : mma_shape<KV_BF16, false>(cols, a, D, s, grid);
-    case CLOVER_B200_F16: return f32 ? mma_shape<KV_F16, true>(cols, a, D, s, grid) : mma_shape<KV_F16, false>(cols, a, D, s, grid);
-    case CLOVER_B200_INT8: return f32 ? mma_shape<KV_I8, true>(cols, a, D, s, grid) : mma_shape<KV_I8, false>(cols, a, D, s, grid);
-    default: return f32 ? mma_shape<KV_E4M3, true>(cols, a, D, s, grid) : mma_shape<KV_E4M3, false>(cols, a, D, s, grid);
+    case CLOVER_B200_BF16: return f32 ? mma_shape<KV_BF16, true>(cols, a, D, s, grid, rings) : mma_shape<KV_BF16, false>(cols, a, D, s, grid, rings);
+    case CLOVER_B200_F16: return f32 ? mma_shape<KV_F16, true>(cols, a, D, s, grid, rings) : mma_shape<KV_F16, false>(cols, a, D, s, grid, rings);
+    case CLOVER_B200_INT8: return f32 ? mma_shape<KV_I8, true>(cols, a, D, s, grid, rings) : mma_shape<KV_I8, false>(cols, a, D, s, grid, rings);
+    default: return f32 ? mma_shape<KV_E4M3, true>(cols, a, D, s, grid, rings) : mma_shape<KV_E4M3, false>(cols, a, D, s, grid, rings);
   }
 }
 
