@@ -236,115 +236,153 @@ attend_generic_kernel(const AttendArgs a) {
 }
 
 // ------------------------------------------------------------------ join
-// One CTA of 4 warps per (segment, column or pair of maps): warp w takes
-// pieces w, w + 4, ... and the warps are joined in shared memory.  A thread
-// owns dims tid and tid + 128.
-constexpr int kJoinWarps = 4;
+// A CTA of 8 warps takes outputs of one segment (a column, or the pair of maps
+// of a head), wpo warps each: 1 where there are outputs enough to fill the GPU,
+// up to 8 where a few columns have hundreds of pieces.  A warp takes every
+// wpo-th piece, kJoinFlight of them in flight; lane l holds dims l, l + 32, ...
+constexpr int kJoinWarps = 8;
 constexpr int kJoinThreads = kJoinWarps * 32;
+constexpr int kJoinFlight = 4;
 
-template <int EPL>
+template <int EPL, int MAPS>
 __global__ void __launch_bounds__(kJoinThreads)
-attend_join_kernel(const AttendArgs a, int n_units) {
-  __shared__ float s_o[2][kJoinWarps][32 * EPL];
-  __shared__ float2 s_ml[2][kJoinWarps];
-  __shared__ float s_sq[kJoinWarps];
+attend_join_kernel(const AttendArgs a, int wpo) {
+  __shared__ float s_o[MAPS][kJoinWarps][32 * EPL];
+  __shared__ float2 s_ml[MAPS][kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int hcmax = a.hkv * a.chunks;
+  const int outs = kJoinWarps / wpo;  // of a CTA
+  const int64_t seg = blockIdx.x;
+  const int b = (int)(seg / hcmax), h = (int)(seg - (int64_t)b * hcmax);
+  const int out = blockIdx.y * outs + warp / wpo, part = warp % wpo;
+  const int c0 = out * MAPS;
+  // the step's layout is final before the attention kernel ran
+  const SeqInfo s = seq_info(a, b);
+  AttendCol ci{0, 0, 0, 0, false};
+  if (h < s.hc && c0 < a.cols) {
+    const int nch = s.hc / a.hkv, kvh = h / nch;
+    ci = attend_col(a, s.row0, s.nq, kvh, (h - kvh * nch) * a.cols + c0);
+  }
   pdl_wait();
   pdl_trigger();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int hcmax = a.hkv * a.chunks;
-  const int units_per_seg = a.cols / a.maps;
-  for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
-    const int seg = u / units_per_seg, c0 = (u - seg * units_per_seg) * a.maps;
-    const int b = seg / hcmax, h = seg - b * hcmax;
-    const SeqInfo s = seq_info(a, b);
-    const int nch = s.hc / a.hkv;
-    if (h >= s.hc) continue;
-    const int kvh = h / nch, chunk = h - kvh * nch;
-    const AttendCol ci = attend_col(a, s.row0, s.nq, kvh, chunk * a.cols + c0);
-    if (!ci.valid) continue;
-    const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * a.D;
-    if (s.n == 0) {  // an empty sequence has no worker
-      for (int d = tid; d < a.D; d += kJoinThreads) attend_store(a, ob + d, 0.f);
-      continue;
-    }
-    const int4 sg = a.seg[seg];
-    if (sg.w <= 1) continue;  // written by its worker
-    // (a worker that gave up waiting leaves its segment's entry unwritten)
-    const int64_t last = sg.y + (int64_t)(sg.w - 1) * sg.z;
-    if (sg.x < 0 || sg.y < 0 || sg.z <= 0 || sg.x >= 2 * a.workers || last >= 2 * a.workers) continue;
-    const int lim = ci.lim;
-    for (int mp = 0; mp < a.maps; ++mp) {
-      float m = -INFINITY, l = 0.f, o[EPL];
+  if (h >= s.hc) return;
+  const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * a.D;
+  if (s.n == 0) {  // an empty sequence has no worker
+    if (ci.valid && part == 0)
+      for (int d = lane; d < a.D; d += 32) attend_store(a, ob + d, 0.f);
+    return;
+  }
+  const int4 sg = a.seg[seg];
+  if (sg.w <= 1) return;  // written by its worker
+  // (a worker that gave up waiting leaves its segment's entry unwritten)
+  const int64_t last = sg.y + (int64_t)(sg.w - 1) * sg.z;
+  if (sg.x < 0 || sg.y < 0 || sg.z <= 0 || sg.x >= 2 * a.workers || last >= 2 * a.workers) return;
+  float o[MAPS][EPL], m[MAPS], l[MAPS];
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) o[e] = 0.f;
-      for (int i = warp; i < sg.w; i += kJoinWarps) {
-        const int64_t slot = i == 0 ? sg.x : sg.y + (int64_t)i * sg.z;
-        const int64_t at = slot * a.cols + c0 + mp;
-        const float2 ml = __ldcg(a.part_ml + at);
-        float x[EPL];
+  for (int mp = 0; mp < MAPS; ++mp) {
+    m[mp] = -INFINITY;
+    l[mp] = 0.f;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          x[e] = lane + 32 * e < a.D ? __ldcg(a.part + at * a.D + lane + 32 * e) : 0.f;
-        const float nm = fmaxf(m, ml.x), uu = nm == -INFINITY ? 0.f : nm;
-        const float f0 = fast_exp2(m - uu), f1 = fast_exp2(ml.x - uu);
-        m = nm;
-        l = fmaf(ml.y, f1, l * f0);
+    for (int e = 0; e < EPL; ++e) o[mp][e] = 0.f;
+  }
+  if (ci.valid) {
+    for (int i0 = part; i0 < sg.w; i0 += wpo * kJoinFlight) {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) o[e] = fmaf(x[e], f1, o[e] * f0);
+      for (int mp = 0; mp < MAPS; ++mp) {
+        float2 ml[kJoinFlight];
+        float x[kJoinFlight][EPL];
+#pragma unroll
+        for (int f = 0; f < kJoinFlight; ++f) {
+          const int i = i0 + f * wpo;
+          const bool ok = i < sg.w;
+          const int64_t slot = i == 0 ? sg.x : sg.y + (int64_t)i * sg.z;
+          const int64_t at = ok ? slot * a.cols + c0 + mp : 0;
+          ml[f] = ok ? __ldcg(a.part_ml + at) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int e = 0; e < EPL; ++e)
+            x[f][e] = ok && lane + 32 * e < a.D ? __ldcg(a.part + at * a.D + lane + 32 * e) : 0.f;
+        }
+        float nm = m[mp];
+#pragma unroll
+        for (int f = 0; f < kJoinFlight; ++f) nm = fmaxf(nm, ml[f].x);
+        const float u = nm == -INFINITY ? 0.f : nm;
+        const float f0 = fast_exp2(m[mp] - u);
+        m[mp] = nm;
+        l[mp] *= f0;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[mp][e] *= f0;
+#pragma unroll
+        for (int f = 0; f < kJoinFlight; ++f) {
+          const float fw = fast_exp2(ml[f].x - u);
+          l[mp] = fmaf(ml[f].y, fw, l[mp]);
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) o[mp][e] = fmaf(x[f][e], fw, o[mp][e]);
+        }
       }
+    }
+  }
+  if (wpo > 1) {
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) s_o[mp][warp][lane + 32 * e] = o[e];
-      if (lane == 0) s_ml[mp][warp] = make_float2(m, l);
+    for (int mp = 0; mp < MAPS; ++mp) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) s_o[mp][warp][lane + 32 * e] = o[mp][e];
+      if (lane == 0) s_ml[mp][warp] = make_float2(m[mp], l[mp]);
     }
     __syncthreads();
-    float w[2][kJoinWarps];
-    for (int mp = 0; mp < a.maps; ++mp) {
-      float M = -INFINITY, L = 0.f;
+    if (part != 0) return;
 #pragma unroll
-      for (int k = 0; k < kJoinWarps; ++k) M = fmaxf(M, s_ml[mp][k].x);
-      const float uu = M == -INFINITY ? 0.f : M;
+    for (int mp = 0; mp < MAPS; ++mp) {
+      for (int k = 1; k < wpo; ++k) {
+        const float2 ml = s_ml[mp][warp + k];
+        const float nm = fmaxf(m[mp], ml.x), u = nm == -INFINITY ? 0.f : nm;
+        const float f0 = fast_exp2(m[mp] - u), f1 = fast_exp2(ml.x - u);
+        m[mp] = nm;
+        l[mp] = fmaf(ml.y, f1, l[mp] * f0);
 #pragma unroll
-      for (int k = 0; k < kJoinWarps; ++k) {
-        w[mp][k] = fast_exp2(s_ml[mp][k].x - uu);
-        L = fmaf(s_ml[mp][k].y, w[mp][k], L);
+        for (int e = 0; e < EPL; ++e) o[mp][e] = fmaf(s_o[mp][warp + k][lane + 32 * e], f1, o[mp][e] * f0);
       }
-      const float inv = attend_inv(L, lim);
-#pragma unroll
-      for (int k = 0; k < kJoinWarps; ++k) w[mp][k] *= inv;
     }
-    const float lam = a.maps == 2 ? a.lam[ci.head] : 0.f;
-    float o[2];
+  }
+  if (!ci.valid) return;
+  const bool any = ci.lim > 0;
+#pragma unroll
+  for (int mp = 0; mp < MAPS; ++mp) {
+    const float inv = attend_inv(l[mp], ci.lim);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[mp][e] = any ? o[mp][e] * inv : 0.f;
+  }
+  if (MAPS == 2) {
+    const float lam = a.lam[ci.head];
     float sq = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int d = tid + e * kJoinThreads;
-      o[e] = 0.f;
-      if (d < a.D && lim > 0) {
-        float o1 = 0.f, o2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < kJoinWarps; ++k) {
-          o1 = fmaf(s_o[0][k][d], w[0][k], o1);
-          if (a.maps == 2) o2 = fmaf(s_o[1][k][d], w[1][k], o2);
-        }
-        o[e] = a.maps == 2 ? diff_value(o1, o2, lam) : o1;
-        sq = fmaf(o[e], o[e], sq);
-      }
+    for (int e = 0; e < EPL; ++e) {
+      o[0][e] = diff_value(o[0][e], o[MAPS - 1][e], lam);
+      sq = fmaf(o[0][e], o[0][e], sq);
     }
-    if (a.maps == 2 && a.norm_w != nullptr) {
+    if (a.norm_w != nullptr) {
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-      if (lane == 0) s_sq[warp] = sq;
-      __syncthreads();
-      const float r = rsqrtf((s_sq[0] + s_sq[1] + s_sq[2] + s_sq[3]) / a.D + a.eps) * a.out_scale;
+      const float r = rsqrtf(sq / a.D + a.eps) * a.out_scale;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (tid + e * kJoinThreads < a.D) o[e] *= r * a.norm_w[tid + e * kJoinThreads];
+      for (int e = 0; e < EPL; ++e)
+        if (lane + 32 * e < a.D) o[0][e] *= r * a.norm_w[lane + 32 * e];
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (tid + e * kJoinThreads < a.D) attend_store(a, ob + tid + e * kJoinThreads, o[e]);
-    __syncthreads();  // shared memory is reused by the next unit
   }
+#pragma unroll
+  for (int e = 0; e < EPL; ++e)
+    if (lane + 32 * e < a.D) attend_store(a, ob + lane + 32 * e, o[0][e]);
+}
+
+template <int MAPS>
+static cudaError_t launch_join(const AttendArgs& a, int sms, cudaStream_t s) {
+  const int64_t segs = (int64_t)a.n_seqs * a.hkv * a.chunks;
+  const int outs = (a.cols + MAPS - 1) / MAPS;  // of a segment
+  int wpo = 1;
+  while (wpo < kJoinWarps && segs * outs * wpo < (int64_t)sms * kJoinWarps * 2) wpo *= 2;
+  const dim3 grid((unsigned)segs, (unsigned)((outs * wpo + kJoinWarps - 1) / kJoinWarps)), block(kJoinThreads);
+  if (a.D <= 64) return launch_pdl(attend_join_kernel<2, MAPS>, grid, block, 0, s, a, wpo);
+  if (a.D <= 128) return launch_pdl(attend_join_kernel<4, MAPS>, grid, block, 0, s, a, wpo);
+  return launch_pdl(attend_join_kernel<8, MAPS>, grid, block, 0, s, a, wpo);
 }
 
 // ------------------------------------------------------------------ append
@@ -634,14 +672,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   rc = sh.mma ? attend_mma(kv_dtype, q_dtype, sh.cols, &a, head_dim, s, nullptr, nullptr)
               : attend_generic(kv_dtype, head_dim, sh.cols, &a, s, sh.sms, nullptr);
   if (rc || sh.whole) return rc;
-  const int64_t units = (int64_t)n_seqs * num_kv_heads * sh.chunks * (sh.cols / maps);
-  const int64_t cap = (int64_t)sh.sms * 16;
-  const dim3 grid((unsigned)(units < cap ? units : cap));
-  const int n = (int)units;
-  cudaError_t e;
-  if (head_dim <= 64) e = launch_pdl(attend_join_kernel<2>, grid, dim3(kJoinThreads), 0, s, a, n);
-  else if (head_dim <= 128) e = launch_pdl(attend_join_kernel<4>, grid, dim3(kJoinThreads), 0, s, a, n);
-  else e = launch_pdl(attend_join_kernel<8>, grid, dim3(kJoinThreads), 0, s, a, n);
+  const cudaError_t e = maps == 2 ? launch_join<2>(a, sh.sms, s) : launch_join<1>(a, sh.sms, s);
   return check_cuda(e, "attend_join launch");
 }
 

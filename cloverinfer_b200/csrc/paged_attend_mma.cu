@@ -22,7 +22,7 @@
 // product (no staging pass):
 //   * K: ldmatrix moves byte pairs, so thread (g, t) of a 16-byte chunk holds
 //     dims 4t .. 4t + 3 of rows g and g + 8.  The order of a dot product's dims
-//     is free: the query fragments take the same order.
+//     is free: the query fragments take the order the conversion gives.
 //   * V: the transposing ldmatrix gives tokens (2t, 2t + 1) x dims (2g, 2g + 1)
 //     in one word; the conversion picks the bytes of one dim, so M row g is dim
 //     2g and row g + 8 dim 2g + 1.
@@ -71,6 +71,10 @@ struct AttendGeom {
   static constexpr int kScales = kEight ? 2 * kTok * 4 : 0;
   static constexpr int kStageB = kTiles + kScales;
   static constexpr int kQTerms = !QF32 ? 1 : KV == KV_BF16 ? 3 : 2;
+  // int8 K codes enter the product 1152 high, and the score's chain starts at
+  // -1152 times the sum of the query: two subtractions less per four codes.  It
+  // costs about 2^-24 * 1152 |sum q| of the score, so not under fp32 queries.
+  static constexpr bool kRawK = KV == KV_I8 && !QF32;
   static constexpr int kPTerms = KV == KV_BF16 && QF32 ? 3 : 2;
   // Warps: 16, 12 or 8 (128, 168 or 255 registers each), as many as hold
   // accumulators, query fragments and about 80 more, with rings at least two
@@ -107,25 +111,36 @@ __device__ __forceinline__ uint32_t hsub2_u(uint32_t a, uint32_t b) {
   asm("sub.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 l;\n\tcvt.u16.u32 l, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(d) : "r"(x));
-  return d;
-}
-
-// Two fp16 pairs from four codes: bytes (0, 1), (2, 3), or with SPLIT the even
-// and the odd bytes (0, 2), (1, 3).
-template <int KV, bool SPLIT>
+// Two fp16 pairs from four codes, in the order bytes (0, 2), (1, 3).  RAW: int8
+// codes stay 1152 higher (the caller's sum takes that off).
+template <int KV, bool RAW = false>
 __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t& lo, uint32_t& hi) {
   if (KV == KV_I8) {
     const uint32_t u = x ^ 0x80808080u;
-    lo = hsub2_u(prmt(u, 0x64646464u, SPLIT ? 0x4240u : 0x4140u), 0x64806480u);
-    hi = hsub2_u(prmt(u, 0x64646464u, SPLIT ? 0x4341u : 0x4342u), 0x64806480u);
+    lo = prmt(u, 0x64646464u, 0x4240u);
+    hi = prmt(u, 0x64646464u, 0x4341u);
+    if (!RAW) {
+      lo = hsub2_u(lo, 0x64806480u);
+      hi = hsub2_u(hi, 0x64806480u);
+    }
   } else {
-    const uint32_t y = SPLIT ? prmt(x, 0u, 0x3120u) : x;
-    lo = e4m3x2_to_f16x2(y);
-    hi = e4m3x2_to_f16x2(y >> 16);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(prmt(x, 0u, 0x3120u)));
   }
+}
+// Two fp16 pairs of e4m3 codes in byte order, (0, 1), (2, 3).
+__device__ __forceinline__ void e4m3_to_f16(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(x));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -166,6 +181,7 @@ struct AttendCols {
   uint32_t q[D / 16][2][G::kQTerms];
   float acc[D / 16][4];
   float m[2], l[2], sc[2];  // sc: score scale in base 2
+  float bias[2];  // int8, 16-bit queries: -1152 * sum of the column's query
   int lim[2];
   int min_lim;  // least limit of the warp's columns
 };
@@ -187,7 +203,9 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
   for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int d = G::kEight ? kk * 16 + (lane & 3) * 4 + i
+      // (the order of K's fragments; int8 words give dims 0, 2 then 1, 3)
+      const int j = KV == KV_I8 ? (i & 1) * 2 + (i >> 1) : i;
+      const int d = G::kEight ? kk * 16 + (lane & 3) * 4 + j
                               : kk * 16 + (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
       const bool in = ci.valid && (a.maps == 1 || (d >= half) == (ci.map == 1));
       x[kk][i] = 0.f;
@@ -217,6 +235,18 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
     split_terms<T, G::kQTerms>(x[kk][0], x[kk][1], c.q[kk][0]);
     split_terms<T, G::kQTerms>(x[kk][2], x[kk][3], c.q[kk][1]);
   }
+  float total = 0.f;
+  if (G::kRawK) {  // of the values as the fragments hold them
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 f = Pack<T>::unpack(c.q[kk][i][0]);
+        total += f.x + f.y;
+      }
+    total += __shfl_xor_sync(0xffffffffu, total, 1);
+    total += __shfl_xor_sync(0xffffffffu, total, 2);
+  }
   // limits and score scales of columns 2t, 2t + 1 from the lanes that hold them
   int lim = ci.valid ? ci.lim : 0;
   if (lim > cap) {  // a row past its sequence's last row
@@ -229,6 +259,7 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
     const int src = ((lane & 3) * 2 + e) * 4;
     c.lim[e] = __shfl_sync(0xffffffffu, lim, src);
     c.sc[e] = a.scale_log2 * __shfl_sync(0xffffffffu, inv, src);
+    c.bias[e] = -1152.f * __shfl_sync(0xffffffffu, total, src);
     c.m[e] = kNoRef;
     c.l[e] = 0.f;
   }
@@ -236,32 +267,32 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
   for (int i = 0; i < D / 16; ++i) c.acc[i][0] = c.acc[i][1] = c.acc[i][2] = c.acc[i][3] = 0.f;
 }
 
-// Fragments of V^T, tokens 16 mt .. 16 mt + 15, for dims 16 i .. 16 i + 15 (8
-// bits: 32 i .. 32 i + 31, two M tiles).
+// Fragments of V^T of 16 tokens for dims 16 i .. 16 i + 15 (8 bits: 32 i ..
+// 32 i + 31, two M tiles).
 template <int KV, int SWZ, int TOK>
 struct VFrag {
   static constexpr int kPer = KV >= KV_I8 ? 2 : 1;
   uint32_t a[kPer][4];
-  __device__ __forceinline__ void load(uint32_t vs, int mt, int i, int lane) {
+  __device__ __forceinline__ void load(uint32_t vs, int i, int lane) {
     const int grp = lane >> 3;
     if (KV >= KV_I8) {
-      const int r = mt * 16 + (lane & 7) + (grp & 1) * 8;
+      const int r = (lane & 7) + (grp & 1) * 8;
       uint32_t x[4];
       ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp >> 1)), x[0], x[1], x[2], x[3]);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
-        codes_to_f16<KV, true>(x[2 * k], a[k][0], a[k][1]);
-        codes_to_f16<KV, true>(x[2 * k + 1], a[k][2], a[k][3]);
+        codes_to_f16<KV>(x[2 * k], a[k][0], a[k][1]);
+        codes_to_f16<KV>(x[2 * k + 1], a[k][2], a[k][3]);
       }
     } else {
-      const int r = mt * 16 + (lane & 7) + (grp >> 1) * 8;
+      const int r = (lane & 7) + (grp >> 1) * 8;
       ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp & 1)), a[0][0], a[0][1], a[0][2], a[0][3]);
     }
   }
-  // Zero the tokens at and past n (of the stage): lo masks tokens 2t, 2t + 1 of
-  // the M tile, hi the tokens 8 later.
-  __device__ __forceinline__ void mask(int mt, int n, int lane) {
-    const int t = mt * 16 + (lane & 3) * 2;
+  // Zero the tokens at and past n: lo masks tokens 2t, 2t + 1, hi the tokens 8
+  // later.
+  __device__ __forceinline__ void mask(int n, int lane) {
+    const int t = (lane & 3) * 2;
     const uint32_t lo = (t < n ? 0xffffu : 0u) | (t + 1 < n ? 0xffff0000u : 0u);
     const uint32_t hi = (t + 8 < n ? 0xffffu : 0u) | (t + 9 < n ? 0xffff0000u : 0u);
 #pragma unroll
@@ -296,92 +327,95 @@ __device__ __forceinline__ bool rows_nonfinite(const uint8_t* v, int r0, int r1,
   return __any_sync(0xffffffffu, bad);
 }
 
-// One stage of one warp.
+// Sixteen tokens of one warp: rows 0 .. 15 at ks / vs (tile row 16 j of the
+// stage: the swizzle repeats every 8 rows), first token tok0, nvalid of them in
+// the context; scales: their K scales, V's kTok floats on.
 template <int KV, bool QF32, int D, int CW>
-__device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, const uint8_t* vgen, const float* scales,
-                                             int tok0, int nvalid, AttendCols<KV, QF32, D, CW>& c, int lane) {
+__device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint8_t* vgen, const float* scales,
+                                            int tok0, int nvalid, AttendCols<KV, QF32, D, CW>& c, int lane) {
   using G = AttendGeom<KV, QF32, D, CW>;
   using T = typename KvMma<KV>::T;
   using VF = VFrag<KV, G::kSwz, G::kTok>;
-  constexpr int KK = D / 16, QT = G::kQTerms, PT = G::kPTerms, MT = G::kTok / 16;
-  constexpr int CH = 2;  // independent chains per score tile
+  constexpr int KK = D / 16, QT = G::kQTerms, PT = G::kPTerms;
   const int g = lane >> 2;
 
-  // ---- S = K . Q^T, times K's scale
-  float s[MT][4];
+  // ---- S = K . Q^T (two chains), times K's scale
+  float ch[2][4], s[4];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    float ch[CH][4];
+  for (int e = 0; e < 4; ++e) {
+    ch[0][e] = G::kRawK ? c.bias[e & 1] : 0.f;
+    ch[1][e] = 0.f;
+  }
+  const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
+  if (G::kEight) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) ch[k][0] = ch[k][1] = ch[k][2] = ch[k][3] = 0.f;
-    const int r = mt * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-    if (G::kEight) {
+    for (int i = 0; i < KK / 2; ++i) {
+      uint32_t x[4];
+      ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, 2 * i + (lane >> 4)), x[0], x[1], x[2], x[3]);
 #pragma unroll
-      for (int i = 0; i < KK / 2; ++i) {
-        uint32_t x[4];
-        ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, 2 * i + (lane >> 4)), x[0], x[1], x[2], x[3]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t a0, a1, a2, a3;
-          codes_to_f16<KV, false>(x[2 * k], a0, a2);
-          codes_to_f16<KV, false>(x[2 * k + 1], a1, a3);
-#pragma unroll
-          for (int q = 0; q < QT; ++q)
-            MmaOp<T>::run(ch[k % CH], a0, a1, a2, a3, c.q[2 * i + k][0][q], c.q[2 * i + k][1][q]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
+      for (int k = 0; k < 2; ++k) {
         uint32_t a0, a1, a2, a3;
-        ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, kk * 2 + (lane >> 4)), a0, a1, a2, a3);
+        if (KV == KV_E4M3) {
+          e4m3_to_f16(x[2 * k], a0, a2);
+          e4m3_to_f16(x[2 * k + 1], a1, a3);
+        } else {
+          codes_to_f16<KV, G::kRawK>(x[2 * k], a0, a2);
+          codes_to_f16<KV, G::kRawK>(x[2 * k + 1], a1, a3);
+        }
 #pragma unroll
         for (int q = 0; q < QT; ++q)
-          MmaOp<T>::run(ch[kk % CH], a0, a1, a2, a3, c.q[kk][0][q], c.q[kk][1][q]);
+          MmaOp<T>::run(ch[k], a0, a1, a2, a3, c.q[2 * i + k][0][q], c.q[2 * i + k][1][q]);
       }
     }
+  } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float ksc = G::kEight ? scales[mt * 16 + g + 8 * h] : 1.f;
+    for (int kk = 0; kk < KK; ++kk) {
+      uint32_t a0, a1, a2, a3;
+      ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, kk * 2 + (lane >> 4)), a0, a1, a2, a3);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float x = ch[0][2 * h + e] + ch[1][2 * h + e];
-        s[mt][2 * h + e] = G::kEight ? x * ksc : x;
-      }
+      for (int q = 0; q < QT; ++q)
+        MmaOp<T>::run(ch[kk & 1], a0, a1, a2, a3, c.q[kk][0][q], c.q[kk][1][q]);
     }
   }
-  // Stages that every column sees whole need no mask.
-  const bool edge = tok0 + G::kTok > c.min_lim;
-  auto masked = [&](int mt, int h, int e) { return edge && tok0 + mt * 16 + g + 8 * h >= c.lim[e]; };
-
-  // ---- the reference: move it when some weight outgrows it.  Each lane looks
-  // at its own scores; only a move takes the columns' maxima over the lanes.
-  float y[MT][4], ve[MT][2];
-  bool moved = false;
+  float vsc[2] = {1.f, 1.f};
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int h = 0; h < 2; ++h) {
+    // V scales under 2^-110 (zero rows; 2^-107 is the least stored) count as that
+    if (G::kEight) vsc[h] = max_nan(scales[G::kTok + g + 8 * h], 7.703719777548943e-34f);
+    const float ksc = G::kEight ? scales[g + 8 * h] : 1.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      ve[mt][h] = 0.f;
-      // 2^ve >= V's scale; scales below 2^-110 count as that (2^-107 is the least stored)
-      if (G::kEight)
-        ve[mt][h] = fmaxf((float)((int)(__float_as_uint(scales[G::kTok + mt * 16 + g + 8 * h]) >> 23 & 255u) - 126),
-                          -110.f);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        y[mt][2 * h + e] = masked(mt, h, e) ? -INFINITY : fmaf(s[mt][2 * h + e], c.sc[e], -c.m[e]);
-        moved |= y[mt][2 * h + e] + ve[mt][h] > 8.f;
-      }
+    for (int e = 0; e < 2; ++e) {
+      const float x = ch[0][2 * h + e] + ch[1][2 * h + e];
+      s[2 * h + e] = G::kEight ? x * ksc : x;
     }
-  if (__any_sync(0xffffffffu, moved)) {
+  }
+  // Steps that every column sees whole need no mask.
+  const bool edge = tok0 + kUnitTok > c.min_lim;
+  auto masked = [&](int h, int e) { return edge && tok0 + g + 8 * h >= c.lim[e]; };
+
+  // ---- weights; the reference moves when one outgrows it.  Each lane looks at
+  // its own; only a move takes the columns' maxima over the lanes.
+  float p[4], w[4], big = 0.f;
+  auto weigh = [&](int h, int e) {
+    const int i = 2 * h + e;
+    p[i] = masked(h, e) ? 0.f : fast_exp2(fmaf(s[i], c.sc[e], -c.m[e]));
+    // (a masked token's scale may be anything: its weight stays 0)
+    w[i] = G::kEight ? (masked(h, e) ? 0.f : p[i] * vsc[h]) : p[i];
+  };
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      weigh(h, e);
+      big = fmaxf(big, w[2 * h + e]);
+    }
+  if (__any_sync(0xffffffffu, big > 256.f)) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (!masked(mt, h, e)) mx = fmaxf(mx, fmaf(s[mt][2 * h + e], c.sc[e], ve[mt][h]));
+      for (int h = 0; h < 2; ++h)
+        if (!masked(h, e)) mx = fmaxf(mx, fmaf(s[2 * h + e], c.sc[e], G::kEight ? fast_log2(vsc[h]) : 0.f));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
       const float nm = fmaxf(c.m[e], mx);
@@ -393,55 +427,39 @@ __device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, const uin
         c.acc[i][e] *= al;
         c.acc[i][2 + e] *= al;
       }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          y[mt][2 * h + e] = masked(mt, h, e) ? -INFINITY : fmaf(s[mt][2 * h + e], c.sc[e], -nm);
+      weigh(0, e);
+      weigh(1, e);
     }
   }
-
-  // ---- weights, split and transposed
-  uint32_t pt[MT][2][PT];
+  c.l[0] += p[0] + p[2];
+  c.l[1] += p[1] + p[3];
+  uint32_t pt[2][PT];  // split and transposed
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int h = 0; h < 2; ++h) {
+    split_terms<T, PT>(w[2 * h], w[2 * h + 1], pt[h]);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float p0 = fast_exp2(y[mt][2 * h]), p1 = fast_exp2(y[mt][2 * h + 1]);
-      c.l[0] += p0;
-      c.l[1] += p1;
-      if (G::kEight) {  // (a masked token's scale may be anything: its weight stays 0)
-        const float vsc = scales[G::kTok + mt * 16 + g + 8 * h];
-        p0 = edge && p0 == 0.f ? 0.f : p0 * vsc;
-        p1 = edge && p1 == 0.f ? 0.f : p1 * vsc;
-      }
-      split_terms<T, PT>(p0, p1, pt[mt][h]);
-#pragma unroll
-      for (int k = 0; k < PT; ++k) pt[mt][h][k] = movm_trans(pt[mt][h][k]);
-    }
+    for (int k = 0; k < PT; ++k) pt[h][k] = movm_trans(pt[h][k]);
+  }
 
   // ---- O^T += V^T . P^T
   if (KV == KV_I8 || !edge) {  // (every int8 code is finite)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int i = 0; i < KK / VF::kPer; ++i) {
+      VF v;
+      v.load(vs, i, lane);
 #pragma unroll
-      for (int i = 0; i < KK / VF::kPer; ++i) {
-        VF v;
-        v.load(vs, mt, i, lane);
+      for (int q = 0; q < PT; ++q)
 #pragma unroll
         for (int k = 0; k < VF::kPer; ++k)
-#pragma unroll
-          for (int q = 0; q < PT; ++q)
-            MmaOp<T>::run(c.acc[i * VF::kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[mt][0][q],
-                          pt[mt][1][q]);
-      }
+          MmaOp<T>::run(c.acc[i * VF::kPer + k], v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[0][q], pt[1][q]);
+    }
     return;
   }
   // Tokens that some column does not see.  Past the context they are masked in
   // V; an infinity or NaN of a later token must not meet the zero weight of an
-  // earlier row (multi-token rows), so a stage that holds one takes its columns
+  // earlier row (multi-token rows), so a step that holds one takes its columns
   // limit by limit, each with V masked from its limit on.
-  const int lo = max(0, c.min_lim - tok0), hi = min(nvalid, G::kTok);
+  const int lo = max(0, c.min_lim - tok0), hi = min(nvalid, kUnitTok);
   const bool plain = !(lo < hi && rows_nonfinite<KV, G::kRow, G::kSwz, G::kTok>(vgen, lo, hi, lane));
   for (int below = 0x7fffffff;;) {
     int top = plain ? tok0 + hi : 0;
@@ -453,23 +471,21 @@ __device__ __forceinline__ void attend_stage(uint32_t ks, uint32_t vs, const uin
       if (top <= tok0) break;
     }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int i = 0; i < KK / VF::kPer; ++i) {
+      VF v;
+      v.load(vs, i, lane);
+      v.mask(top - tok0, lane);
 #pragma unroll
-      for (int i = 0; i < KK / VF::kPer; ++i) {
-        VF v;
-        v.load(vs, mt, i, lane);
-        v.mask(mt, top - tok0, lane);
+      for (int k = 0; k < VF::kPer; ++k) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < VF::kPer; ++k) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < PT; ++q)
+          MmaOp<T>::run(x, v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[0][q], pt[1][q]);
 #pragma unroll
-          for (int q = 0; q < PT; ++q)
-            MmaOp<T>::run(x, v.a[k][0], v.a[k][1], v.a[k][2], v.a[k][3], pt[mt][0][q], pt[mt][1][q]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (plain || c.lim[e & 1] == top) c.acc[i * VF::kPer + k][e] += x[e];
-        }
+        for (int e = 0; e < 4; ++e)
+          if (plain || c.lim[e & 1] == top) c.acc[i * VF::kPer + k][e] += x[e];
       }
+    }
     if (plain) break;
     below = top;
   }
@@ -775,11 +791,17 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
     if (cols) {
       const uint32_t ks = ring_s + st * G::kTiles;
-      const int tok0 = cur.jj * G::kTok;
-      attend_stage<KV, QF32, D, CW>(
-          ks, ks + G::kTile, smem + ring * G::kRingTiles + st * G::kTiles + G::kTile,
-          reinterpret_cast<const float*>(smem_sc + (ring * STAGES + st) * G::kScales), tok0, cur.s.ctx - tok0, c,
-          lane);
+      const uint8_t* vgen = smem + ring * G::kRingTiles + st * G::kTiles + G::kTile;
+      const float* sc = reinterpret_cast<const float*>(smem_sc + (ring * STAGES + st) * G::kScales);
+      // (a loop, not unrolled: half the code in the instruction cache)
+#pragma unroll 1
+      for (int u = 0; u < G::kSubs; ++u) {
+        const int tok0 = cur.jj * G::kTok + u * kUnitTok;
+        if (tok0 >= cur.s.ctx) break;
+        attend_step<KV, QF32, D, CW>(ks + u * kUnitTok * G::kSwz, ks + G::kTile + u * kUnitTok * G::kSwz,
+                                     vgen + u * kUnitTok * G::kSwz, sc + u * kUnitTok, tok0, cur.s.ctx - tok0, c,
+                                     lane);
+      }
     }
     __syncwarp();
     if (CW > 1 && cw > 0 && lane == 0) mbar_arrive(empty + st * 8);
