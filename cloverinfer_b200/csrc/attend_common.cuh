@@ -18,7 +18,9 @@
 //   * ranged launches, where aligned pieces would leave workers idle (more
 //     than a sixth longer than an even share: many segments, or very ragged
 //     ones): units are numbered sequence-major, then segment, then along the
-//     context, and worker w takes [w per, (w + 1) per).  A range meets at most
+//     context, with kSegCost empty numbers before a segment's first unit (a
+//     worker with many short segments else takes far longer than one inside a
+//     long one), and worker w takes [w per, (w + 1) per).  A range meets at most
 //     two segments it does not hold whole: its first (a piece that starts inside
 //     the segment, partial slot 2w) and its last (a piece with the segment's
 //     first unit, slot 2w + 1).  The workspace is 2 slots per worker whatever
@@ -38,7 +40,8 @@ namespace clover {
 constexpr int kUnitTok = 16;     // a unit is a multiple of this
 constexpr int kAttendWarps = 4;  // workers of a generic CTA
 constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kAttendMinTok = 128;  // a worker's least range
+constexpr int kAttendMinTok = 64;   // a worker's least range (measured: 32 requests of 300 tokens, 19.2 us at 128)
+constexpr int kSegCost = 4;         // what a segment costs beside its units (queries, output), in units
 constexpr int kAttendMaxPerSm = 16; // generic workers per SM
 
 struct AttendArgs {
@@ -47,6 +50,7 @@ struct AttendArgs {
   const void* q;
   int64_t q_stride;
   int32_t q_dtype;
+  int32_t q_vec;  // query rows are 16-byte aligned
   const void* kc;
   const void* vc;
   const float* ks;  // [num_blocks, num_kv_heads, block_size]; null: no scales
@@ -188,8 +192,9 @@ struct Cursor {
     if (a.whole) return ++jj < s.n || seek(a, (int64_t)seg0 + a.workers);
     if (--left <= 0) return false;
     if (++jj < s.n) return true;
+    if ((left -= kSegCost) <= 0) return false;
     jj = 0;
-    seg0 += s.n;
+    seg0 += s.n + kSegCost;
     if (++h < s.hc) return true;
     h = 0;
     do {
@@ -219,6 +224,13 @@ struct AttendSplit {
   bool aligned;
 };
 
+// Range k of those tried for aligned pieces: a ranged worker's `even` numbers
+// hold even - kSegCost units and one segment's cost.
+__device__ __forceinline__ int attend_try(int even, int k) {
+  const int u = even - kSegCost;
+  return u + (u * k + 31) / 32;
+}
+
 // Every CTA counts the step's units by itself (thread i takes sequences
 // [i c, (i + 1) c)) and finds where its workers (r * gridDim.x + blockIdx.x)
 // start; all threads call it.
@@ -227,11 +239,15 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int c = (a.n_seqs + NW * 32 - 1) / (NW * 32);
   const int b0 = min(a.n_seqs, tid * c), b1 = min(a.n_seqs, b0 + c);
+  SeqInfo kept{0, 0, 0, 0, 0};  // of the one sequence of a thread (c = 1)
+  auto info = [&](int b) { return c == 1 ? kept : seq_info(a, b); };
+  // numbers of a sequence in a ranged launch
+  auto numbers = [](const SeqInfo& s) { return s.n > 0 ? s.hc * (s.n + kSegCost) : 0; };
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const SeqInfo s = seq_info(a, b);
-    if (blockIdx.x == 0) attend_check_seq(a, s);
-    mine += s.n * s.hc;
+    kept = seq_info(a, b);
+    if (blockIdx.x == 0) attend_check_seq(a, kept);
+    mine += numbers(kept);
   }
   int x = __reduce_add_sync(0xffffffffu, mine);
   if (lane == 0) p.sum[warp][0] = x;
@@ -240,15 +256,17 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
   AttendSplit sp{0, 0, false};
 #pragma unroll
   for (int w = 0; w < NW; ++w) sp.total += p.sum[w][0];
-  const int even = max((sp.total + a.workers - 1) / a.workers, kAttendMinTok >> a.unit_log2);
+  // an even share (aligned pieces pay for their segment themselves); a range
+  // has to hold more than the cost of a segment
+  const int even = max((sp.total + a.workers - 1) / a.workers, kSegCost + (kAttendMinTok >> a.unit_log2));
   int pieces[kAlignTries];
 #pragma unroll
   for (int k = 0; k < kAlignTries; ++k) pieces[k] = 0;
   for (int b = b0; b < b1; ++b) {
-    const SeqInfo s = seq_info(a, b);
+    const SeqInfo s = info(b);
 #pragma unroll
     for (int k = 0; k < kAlignTries; ++k) {
-      const int per = even + (even * k + 31) / 32;
+      const int per = attend_try(even, k);
       pieces[k] += s.hc * ((s.n + per - 1) / per);
     }
   }
@@ -267,7 +285,7 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
     for (int w = 0; w < NW; ++w) all += p.sum[w][k + 1];
     if (!sp.aligned && all <= a.workers) {
       sp.aligned = true;
-      sp.per = even + (even * k + 31) / 32;
+      sp.per = attend_try(even, k);
       mine = pieces[k];
       col = k + 1;
     }
@@ -286,9 +304,9 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
     if (u0 < before || u0 >= before + mine) continue;
     int at = before;
     for (int b = b0; b < b1; ++b) {
-      const SeqInfo s = seq_info(a, b);
+      const SeqInfo s = info(b);
       const int kp = (s.n + sp.per - 1) / sp.per;
-      const int u = s.hc * (sp.aligned ? kp : s.n);
+      const int u = sp.aligned ? s.hc * kp : numbers(s);
       if (u0 < at + u) {
         const int off = (int)(u0 - at);
         p.start[k][0] = b;
@@ -300,11 +318,12 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
           p.seg0[k] = 0;
           if (i * len >= s.n) p.start[k][0] = -1;  // (rounding left the last piece empty)
         } else {
-          const int h = off / s.n;
+          const int h = off / (s.n + kSegCost), in = off - h * (s.n + kSegCost);
           p.start[k][1] = h;
-          p.start[k][2] = off - h * s.n;
-          p.start[k][3] = (int)min((int64_t)sp.per, sp.total - u0);
-          p.seg0[k] = at + h * s.n;
+          p.start[k][2] = max(0, in - kSegCost);
+          p.start[k][3] = (int)min((int64_t)sp.per, sp.total - u0) - max(0, kSegCost - in);
+          p.seg0[k] = at + h * (s.n + kSegCost);
+          if (p.start[k][3] <= 0) p.start[k][0] = -1;  // (the batch ends before a unit)
         }
         break;
       }
@@ -340,8 +359,8 @@ __device__ __forceinline__ void attend_record(const AttendArgs& a, const AttendS
     const int kp = (s.n + sp.per - 1) / sp.per, len = (s.n + kp - 1) / kp;
     e = make_int4(wid, wid, s.hc, (s.n + len - 1) / len);
   } else {
-    const int fw = seg0 / sp.per;
-    e = make_int4(2 * fw + 1, 2 * fw, 2, (seg0 + s.n - 1) / sp.per - fw + 1);
+    const int first = seg0 + kSegCost, fw = first / sp.per;
+    e = make_int4(2 * fw + 1, 2 * fw, 2, (first + s.n - 1) / sp.per - fw + 1);
   }
   a.seg[(int64_t)b * (a.hkv * a.chunks) + h] = e;
 }

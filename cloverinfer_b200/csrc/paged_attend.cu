@@ -539,7 +539,7 @@ static int attend_shape(int n_seqs, int n_rows, int max_q, int max_ctx, int hq, 
   const int64_t units = ((int64_t)max_ctx + (1 << p->unit_log2) - 1) >> p->unit_log2;
   const int64_t least = kAttendMinTok >> p->unit_log2;  // units of a worker's least range
   if (chunks > 65535 || (int64_t)n_seqs * hkv * chunks > INT32_MAX / 64 ||
-      (int64_t)n_seqs * hkv * chunks * (units > 0 ? units : 1) > INT32_MAX)
+      (int64_t)n_seqs * hkv * chunks * (units + kSegCost) > INT32_MAX)
     return set_error(CLOVER_B200_ERR_UNSUPPORTED, "attend: batch too large");
   p->chunks = (int)chunks;
   // Short contexts: a segment is at most two ranges' least work; splitting it
@@ -632,6 +632,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   a.group = num_q_heads / num_kv_heads;
   a.maps = maps;
   a.D = head_dim;
+  a.q_vec = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(q_row_stride * (q_dtype == CLOVER_B200_F32 ? 4 : 2))) & 15) == 0;
   a.bs = block_size;
   a.num_blocks = num_blocks;
   a.scale_log2 = score_scale * 1.4426950408889634f;

@@ -199,22 +199,54 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
   const int64_t qb = (int64_t)ci.row * a.q_stride + (int64_t)ci.head * D;
   float x[D / 16][4];
   uint32_t big = 0;
+  // the lane's dims of a 16-dim group, in runs of 4 (8-bit caches) or 2
+  constexpr int kRun = G::kEight ? 4 : 2;
+  const bool f16 = a.q_dtype == CLOVER_B200_F16;
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // (the order of K's fragments; int8 words give dims 0, 2 then 1, 3)
-      const int j = KV == KV_I8 ? (i & 1) * 2 + (i >> 1) : i;
-      const int d = G::kEight ? kk * 16 + (lane & 3) * 4 + j
-                              : kk * 16 + (lane & 3) * 2 + (i & 1) + (i >> 1) * 8;
-      const bool in = ci.valid && (a.maps == 1 || (d >= half) == (ci.map == 1));
-      x[kk][i] = 0.f;
-      if (in) {
-        if (QF32) x[kk][i] = static_cast<const float*>(a.q)[qb + d];
-        else if (a.q_dtype == CLOVER_B200_F16) x[kk][i] = __half2float(static_cast<const __half*>(a.q)[qb + d]);
-        else x[kk][i] = __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[qb + d]);
+    for (int j = 0; j < 4; j += kRun) {
+      const int d = kk * 16 + (lane & 3) * kRun + j * (8 / kRun);
+      const bool in = ci.valid && (a.maps == 1 || (d >= half) == (ci.map == 1));  // (a run lies in one half)
+      float v[kRun];
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) v[i] = 0.f;
+      if (in && QF32) {
+        const float* src = static_cast<const float*>(a.q) + qb + d;
+        if (a.q_vec && kRun == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(src);
+          v[0] = f.x, v[1] = f.y, v[kRun - 2] = f.z, v[kRun - 1] = f.w;
+        } else if (a.q_vec) {
+          const float2 f = *reinterpret_cast<const float2*>(src);
+          v[0] = f.x, v[1] = f.y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRun; ++i) v[i] = src[i];
+        }
+      } else if (in) {
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + qb + d;
+        uint32_t w[2] = {0, 0};
+        if (a.q_vec && kRun == 4) {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          w[0] = u.x, w[1] = u.y;
+        } else if (a.q_vec) {
+          w[0] = *reinterpret_cast<const uint32_t*>(src);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRun; i += 2) w[i / 2] = src[i] | ((uint32_t)src[i + 1] << 16);
+        }
+#pragma unroll
+        for (int i = 0; i < kRun; i += 2) {
+          const float2 f = f16 ? Pack<__half>::unpack(w[i / 2]) : Pack<__nv_bfloat16>::unpack(w[i / 2]);
+          v[i] = f.x, v[i + 1] = f.y;
+        }
       }
-      big = max(big, abs_bits(x[kk][i]));
+      // the order of K's fragments: int8 words give dims 0, 2 then 1, 3
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        x[kk][j + i] = v[KV == KV_I8 ? (i & 1) * 2 + (i >> 1) : i];
+        big = max(big, abs_bits(v[i]));
+      }
     }
   }
   float inv = 1.f;
@@ -707,19 +739,19 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __shared__ AttendPlan<G::kWarps, RINGS> plan;
   __shared__ int s_stop;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < RINGS * STAGES; ++i) {
-      mbar_init(smem_addr(&s_full[i]), G::kEight ? 33 : 1);  // the tiles, and each lane's scales
-      mbar_init(smem_addr(&s_empty[i]), 1);                  // the ring's other warp
-    }
+  // after a bounded wait gave up anywhere, later launches stop at once
+  if (threadIdx.x == 0)
+    s_stop = a.status != nullptr && (*(volatile int32_t*)a.status & CLOVER_B200_DEV_TIMEOUT);
+  for (int i = threadIdx.x; i < RINGS * STAGES; i += G::kThreads) {
+    mbar_init(smem_addr(&s_full[i]), G::kEight ? 33 : 1);  // the tiles, and each lane's scales
+    mbar_init(smem_addr(&s_empty[i]), 1);                  // the ring's other warp
     fence_mbar_init();
+  }
+  if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
   pdl_wait();
-  // after a bounded wait gave up anywhere, later launches stop at once
-  if (threadIdx.x == 0)
-    s_stop = a.status != nullptr && (*(volatile int32_t*)a.status & CLOVER_B200_DEV_TIMEOUT);
   __syncthreads();
   if (s_stop) return;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
