@@ -328,19 +328,21 @@ def decode_step(out, q, k_cache, v_cache, k_new, v_new, block_tables, query_star
 
 
 # ---------------------------------------------------------------- step plan, 8-bit caches, differential decode
-def _one_device(what, *ts) -> torch.device:
-    """The device all given tensors live on (None is skipped)."""
-    dev = ts[0].device
+def _one_device(what, *ts) -> int:
+    """Ordinal of the CUDA device all given tensors live on (None is skipped)."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and (t.device != dev or not t.is_cuda):
-            raise ValueError(f"{what}: tensors must be on one CUDA device, got {t.device} beside {dev}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors must be on one CUDA device, got {t.device} beside {ts[0].device}")
+    if dev < 0:
+        raise ValueError(f"{what}: takes CUDA tensors, got {ts[0].device}")
     return dev
 
 
-def _call_on(dev: torch.device, fn, *args) -> int:
+def _call_on(dev: int, fn, *args) -> int:
     """Call a launching entry point with its tensors' device current and its
     current stream as the last argument."""
-    if dev.index == torch.cuda.current_device():
+    if dev == torch.cuda.current_device():
         return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
     with torch.cuda.device(dev):
         return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
@@ -348,7 +350,7 @@ def _call_on(dev: torch.device, fn, *args) -> int:
 
 def _index_i32(what, *ts) -> None:
     for t in ts:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
             raise TypeError(f"{what}: index tensors must be contiguous int32")
 
 
@@ -495,7 +497,7 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
     if rows == 0 or n_seqs == 0:
         return
     if workspace is None:
-        key = (dev.index, n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d, bs, k_cache.dtype,
+        key = (dev, n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d, bs, k_cache.dtype,
                q.dtype, diff)
         need = _attend_ws.get(key)
         if need is None:
@@ -505,7 +507,7 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
                 _attend_ws.clear()
             _attend_ws[key] = need
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     args = (out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), dtype_code(q.dtype),
             k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales),
             dtype_code(k_cache.dtype), nb, bs, _ptr(k_new), _ptr(v_new),

@@ -18,7 +18,7 @@
 //   * ranged launches, where aligned pieces would leave workers idle (more
 //     than a sixth longer than an even share: many segments, or very ragged
 //     ones): units are numbered sequence-major, then segment, then along the
-//     context, with kSegCost empty numbers before a segment's first unit (a
+//     context, with the segment's cost in empty numbers before its first unit (a
 //     worker with many short segments else takes far longer than one inside a
 //     long one), and worker w takes [w per, (w + 1) per).  A range meets at most
 //     two segments it does not hold whole: its first (a piece that starts inside
@@ -41,7 +41,7 @@ constexpr int kUnitTok = 16;     // a unit is a multiple of this
 constexpr int kAttendWarps = 4;  // workers of a generic CTA
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kAttendMinTok = 64;   // a worker's least range (measured: 32 requests of 300 tokens, 19.2 us at 128)
-constexpr int kSegCost = 4;         // what a segment costs beside its units (queries, output), in units
+constexpr int kSegCostTok = 128;    // what a segment costs beside its units (queries, output), as tokens
 constexpr int kAttendMaxPerSm = 16; // generic workers per SM
 
 struct AttendArgs {
@@ -62,6 +62,7 @@ struct AttendArgs {
   const int32_t* ctx;
   int32_t n_seqs, n_rows, max_ctx;
   int32_t unit_log2;  // log2 of a unit's tokens
+  int32_t seg_cost;   // of a segment, in units
   int32_t hq, hkv, group, maps;  // maps: 1, or 2 for differential attention
   int32_t D, bs;
   int64_t num_blocks;
@@ -192,9 +193,9 @@ struct Cursor {
     if (a.whole) return ++jj < s.n || seek(a, (int64_t)seg0 + a.workers);
     if (--left <= 0) return false;
     if (++jj < s.n) return true;
-    if ((left -= kSegCost) <= 0) return false;
+    if ((left -= a.seg_cost) <= 0) return false;
     jj = 0;
-    seg0 += s.n + kSegCost;
+    seg0 += s.n + a.seg_cost;
     if (++h < s.hc) return true;
     h = 0;
     do {
@@ -212,7 +213,7 @@ struct Cursor {
 constexpr int kAlignTries = 6;  // aligned ranges up to 5/32 longer than an even share
 template <int NW, int R>
 struct AttendPlan {
-  int sum[NW][kAlignTries + 1];  // per warp: units, then pieces at each range tried
+  int sum[NW][kAlignTries + 2];  // per warp: numbers, pieces at each range tried, units
   int start[R][4];               // sequence, segment, first unit, units (ranged: flat number of the segment)
   int seg0[R];
 };
@@ -221,19 +222,19 @@ struct AttendPlan {
 // are aligned.
 struct AttendSplit {
   int per, total;
+  int quota;  // workers of a CTA that have work
   bool aligned;
 };
 
-// Range k of those tried for aligned pieces: a ranged worker's `even` numbers
-// hold even - kSegCost units and one segment's cost.
-__device__ __forceinline__ int attend_try(int even, int k) {
-  const int u = even - kSegCost;
-  return u + (u * k + 31) / 32;
-}
+// Worker r of this CTA: the CTA's workers are consecutive, so every SM has the
+// same share of the step; r >= quota has no work.
+__device__ __forceinline__ int attend_worker(const AttendSplit& sp, int r) { return blockIdx.x * sp.quota + r; }
+
+// Range k of those tried for aligned pieces.
+__device__ __forceinline__ int attend_try(int even, int k) { return even + (even * k + 31) / 32; }
 
 // Every CTA counts the step's units by itself (thread i takes sequences
-// [i c, (i + 1) c)) and finds where its workers (r * gridDim.x + blockIdx.x)
-// start; all threads call it.
+// [i c, (i + 1) c)) and finds where its workers start; all threads call it.
 template <int NW, int R>
 __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPlan<NW, R>& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -242,23 +243,34 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
   SeqInfo kept{0, 0, 0, 0, 0};  // of the one sequence of a thread (c = 1)
   auto info = [&](int b) { return c == 1 ? kept : seq_info(a, b); };
   // numbers of a sequence in a ranged launch
-  auto numbers = [](const SeqInfo& s) { return s.n > 0 ? s.hc * (s.n + kSegCost) : 0; };
-  int mine = 0;
+  auto numbers = [&](const SeqInfo& s) { return s.n > 0 ? s.hc * (s.n + a.seg_cost) : 0; };
+  int mine = 0, units = 0;
   for (int b = b0; b < b1; ++b) {
     kept = seq_info(a, b);
     if (blockIdx.x == 0) attend_check_seq(a, kept);
     mine += numbers(kept);
+    units += kept.n * kept.hc;
   }
   int x = __reduce_add_sync(0xffffffffu, mine);
-  if (lane == 0) p.sum[warp][0] = x;
+  units = __reduce_add_sync(0xffffffffu, units);
+  if (lane == 0) {
+    p.sum[warp][0] = x;
+    p.sum[warp][kAlignTries + 1] = units;
+  }
   if (tid < R) p.start[tid][0] = -1;
   __syncthreads();
-  AttendSplit sp{0, 0, false};
+  AttendSplit sp{0, 0, R, false};
+  int all_units = 0;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) sp.total += p.sum[w][0];
-  // an even share (aligned pieces pay for their segment themselves); a range
-  // has to hold more than the cost of a segment
-  const int even = max((sp.total + a.workers - 1) / a.workers, kSegCost + (kAttendMinTok >> a.unit_log2));
+  for (int w = 0; w < NW; ++w) {
+    sp.total += p.sum[w][0];
+    all_units += p.sum[w][kAlignTries + 1];
+  }
+  // even shares: of the numbers (a range has to hold more than a segment's
+  // cost), and of the units for aligned pieces
+  const int least = kAttendMinTok >> a.unit_log2;
+  const int even = max((sp.total + a.workers - 1) / a.workers, a.seg_cost + least);
+  const int even_units = max((all_units + a.workers - 1) / a.workers, least);
   int pieces[kAlignTries];
 #pragma unroll
   for (int k = 0; k < kAlignTries; ++k) pieces[k] = 0;
@@ -266,7 +278,7 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
     const SeqInfo s = info(b);
 #pragma unroll
     for (int k = 0; k < kAlignTries; ++k) {
-      const int per = attend_try(even, k);
+      const int per = attend_try(even_units, k);
       pieces[k] += s.hc * ((s.n + per - 1) / per);
     }
   }
@@ -277,6 +289,7 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
   }
   __syncthreads();
   int col = 0;  // of p.sum: what is numbered
+  int used = (sp.total + even - 1) / even;  // workers
   sp.per = even;
 #pragma unroll
   for (int k = 0; k < kAlignTries; ++k) {
@@ -285,11 +298,13 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
     for (int w = 0; w < NW; ++w) all += p.sum[w][k + 1];
     if (!sp.aligned && all <= a.workers) {
       sp.aligned = true;
-      sp.per = attend_try(even, k);
+      sp.per = attend_try(even_units, k);
       mine = pieces[k];
       col = k + 1;
+      used = all;
     }
   }
+  sp.quota = min(R, max(1, (used + (int)gridDim.x - 1) / (int)gridDim.x));
   int incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -298,8 +313,8 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
   }
   int before = incl - mine;
   for (int w = 0; w < warp; ++w) before += p.sum[w][col];
-  for (int k = 0; k < R; ++k) {
-    const int wid = k * gridDim.x + blockIdx.x;
+  for (int k = 0; k < sp.quota; ++k) {
+    const int wid = attend_worker(sp, k);
     const int64_t u0 = sp.aligned ? wid : (int64_t)wid * sp.per;
     if (u0 < before || u0 >= before + mine) continue;
     int at = before;
@@ -318,11 +333,11 @@ __device__ __forceinline__ AttendSplit attend_plan(const AttendArgs& a, AttendPl
           p.seg0[k] = 0;
           if (i * len >= s.n) p.start[k][0] = -1;  // (rounding left the last piece empty)
         } else {
-          const int h = off / (s.n + kSegCost), in = off - h * (s.n + kSegCost);
+          const int h = off / (s.n + a.seg_cost), in = off - h * (s.n + a.seg_cost);
           p.start[k][1] = h;
-          p.start[k][2] = max(0, in - kSegCost);
-          p.start[k][3] = (int)min((int64_t)sp.per, sp.total - u0) - max(0, kSegCost - in);
-          p.seg0[k] = at + h * (s.n + kSegCost);
+          p.start[k][2] = max(0, in - a.seg_cost);
+          p.start[k][3] = (int)min((int64_t)sp.per, sp.total - u0) - max(0, a.seg_cost - in);
+          p.seg0[k] = at + h * (s.n + a.seg_cost);
           if (p.start[k][3] <= 0) p.start[k][0] = -1;  // (the batch ends before a unit)
         }
         break;
@@ -359,7 +374,7 @@ __device__ __forceinline__ void attend_record(const AttendArgs& a, const AttendS
     const int kp = (s.n + sp.per - 1) / sp.per, len = (s.n + kp - 1) / kp;
     e = make_int4(wid, wid, s.hc, (s.n + len - 1) / len);
   } else {
-    const int first = seg0 + kSegCost, fw = first / sp.per;
+    const int first = seg0 + a.seg_cost, fw = first / sp.per;
     e = make_int4(2 * fw + 1, 2 * fw, 2, (first + s.n - 1) / sp.per - fw + 1);
   }
   a.seg[(int64_t)b * (a.hkv * a.chunks) + h] = e;

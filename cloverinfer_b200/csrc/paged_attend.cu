@@ -39,9 +39,9 @@ __global__ void __launch_bounds__(kAttendThreads)
 attend_generic_kernel(const AttendArgs a) {
   __shared__ AttendPlan<kAttendWarps, kAttendWarps> plan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int wid = warp * gridDim.x + blockIdx.x;
+  int wid = warp * gridDim.x + blockIdx.x;
   pdl_wait();
-  AttendSplit sp{1, 0, false};
+  AttendSplit sp{1, 0, 0, false};
   Cursor cur;
   int seg = 0;  // whole launches: the worker's segment (empty ones too: their zeros)
   const int hcmax = a.hkv * a.chunks;
@@ -49,6 +49,7 @@ attend_generic_kernel(const AttendArgs a) {
     sp = attend_plan<kAttendWarps, kAttendWarps>(a, plan);
     pdl_trigger();
     if (!attend_start(a, plan, warp, cur)) return;
+    wid = attend_worker(sp, warp);
   } else {
     seg = wid - a.workers;
   }
@@ -539,7 +540,7 @@ static int attend_shape(int n_seqs, int n_rows, int max_q, int max_ctx, int hq, 
   const int64_t units = ((int64_t)max_ctx + (1 << p->unit_log2) - 1) >> p->unit_log2;
   const int64_t least = kAttendMinTok >> p->unit_log2;  // units of a worker's least range
   if (chunks > 65535 || (int64_t)n_seqs * hkv * chunks > INT32_MAX / 64 ||
-      (int64_t)n_seqs * hkv * chunks * (units + kSegCost) > INT32_MAX)
+      (int64_t)n_seqs * hkv * chunks * (units + kSegCostTok) > INT32_MAX)
     return set_error(CLOVER_B200_ERR_UNSUPPORTED, "attend: batch too large");
   p->chunks = (int)chunks;
   // Short contexts: a segment is at most two ranges' least work; splitting it
@@ -637,6 +638,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
   a.num_blocks = num_blocks;
   a.scale_log2 = score_scale * 1.4426950408889634f;
   a.unit_log2 = sh.unit_log2;
+  a.seg_cost = kSegCostTok >> sh.unit_log2;
   a.cols = sh.cols;
   a.chunks = sh.chunks;
   a.whole = sh.whole;

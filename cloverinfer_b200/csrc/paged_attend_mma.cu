@@ -756,16 +756,14 @@ attend_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (s_stop) return;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_sc = smem + RINGS * G::kRingTiles;
-  AttendSplit sp{1, 0, false};
+  AttendSplit sp{1, 0, 0, false};
   if (!a.whole) {
     sp = attend_plan<G::kWarps, RINGS>(a, plan);
     pdl_trigger();
   }
 
-  // ring r of this CTA is worker r * gridDim.x + blockIdx.x: few workers spread
-  // over the SMs
   const int ring = warp / CW, cw = warp % CW;
-  const int wid = ring * gridDim.x + blockIdx.x;
+  const int wid = a.whole ? ring * gridDim.x + blockIdx.x : attend_worker(sp, ring);
   if (a.whole && cw == 0) {
     // rows of empty sequences have no unit: their zeros are written here
     const int hcmax = a.hkv * a.chunks;

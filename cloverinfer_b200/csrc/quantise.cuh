@@ -44,14 +44,12 @@ __device__ __forceinline__ uint32_t encode4(const float* x, float factor) {
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * factor, x[3] * factor), __NV_SATFINITE, __NV_E4M3);
     return (lo & 0xffffu) | (hi << 16);
   }
-  uint32_t w = 0;
+  // Adding 1.5 * 2^23 leaves the value rounded to nearest even in the low bits
+  // (|x factor| is at most 127 (1 + 3 * 2^-24): 127 after rounding, no clamp).
+  uint32_t v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    int v = __float2int_rn(x[i] * factor);
-    v = max(-127, min(127, v));
-    w |= (uint32_t)(v & 0xff) << (8 * i);
-  }
-  return w;
+  for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], factor), 12582912.f));
+  return __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
 }
 
 template <bool FP8>

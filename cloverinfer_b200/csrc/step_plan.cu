@@ -14,12 +14,13 @@
 //
 // Bound: launch latency and three dependent loads (rows, lengths, block ids)
 // for a decode step; for admissions of whole prompts the 12 bytes written per
-// token.  One thread-block cluster: every CTA scans all items by itself (into
+// token (12 bytes of 228k tokens: 35 us from 8 CTAs of 512 threads, a round of
+// dependent loads per 16k tokens; 16 CTAs of 1024 threads: 11).  One thread-block
+// cluster: every CTA scans all items by itself (into
 // shared memory) and takes its share of the tokens, and the state that the
 // scans read (lengths, table lengths, stack top) is committed after the
 // cluster barrier, so no global counter or scratch memory is needed.
 #include <cooperative_groups.h>
-#include <cub/block/block_scan.cuh>
 
 #include "common.cuh"
 
@@ -27,7 +28,7 @@ namespace clover {
 
 namespace cg = cooperative_groups;
 
-constexpr int kPlanThreads = 512;
+constexpr int kPlanSmall = 256, kPlanLarge = 1024;  // threads: decode steps, admissions
 constexpr int kPlanMaxItems = 8192;
 constexpr int kPlanMaxRows = 1 << 18;
 constexpr int kPlanGroup = 4;  // consecutive tokens of one thread
@@ -49,6 +50,7 @@ struct PlanArgs {
   int32_t* ctx;
   int64_t* slots;
   int32_t max_tokens;
+  int32_t vec;  // ctx and slots are 16-byte aligned
   int32_t* status;
 };
 
@@ -62,10 +64,11 @@ __device__ __forceinline__ int plan_find(const int32_t* off, int n, int32_t k) {
   return lo;
 }
 
+template <int kPlanThreads>
 __global__ void __launch_bounds__(kPlanThreads)
 plan_step_kernel(const PlanArgs a) {
-  using Scan = cub::BlockScan<int64_t, kPlanThreads>;
-  __shared__ typename Scan::TempStorage tmp;
+  constexpr int NW = kPlanThreads / 32;
+  __shared__ int64_t s_sum[2][NW];
   __shared__ int32_t s_bad;
   extern __shared__ int32_t s_dyn[];
   int32_t* s_tok = s_dyn;            // [n + 1] first token
@@ -110,11 +113,32 @@ plan_step_kernel(const PlanArgs a) {
       s_have[i] = have;
     }
     if (bad) atomicOr(&s_bad, bad);
-    // both sums fit 32 bits each whenever the plan is accepted
-    int64_t off_t, off_p, tot_t, tot_p;
-    Scan(tmp).ExclusiveSum(tok, off_t, tot_t);
+    // exclusive sums over the CTA (64 bits: an unacceptable plan may overflow 32)
+    int64_t in_t = tok, in_p = pop;
+    const int lane = tid & 31, warp = tid >> 5;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, in_t, off), z = __shfl_up_sync(0xffffffffu, in_p, off);
+      if (lane >= off) {
+        in_t += y;
+        in_p += z;
+      }
+    }
+    if (lane == 31) {
+      s_sum[0][warp] = in_t;
+      s_sum[1][warp] = in_p;
+    }
     __syncthreads();
-    Scan(tmp).ExclusiveSum(pop, off_p, tot_p);
+    int64_t off_t = in_t - tok, off_p = in_p - pop, tot_t = 0, tot_p = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) {
+        off_t += s_sum[0][w];
+        off_p += s_sum[1][w];
+      }
+      tot_t += s_sum[0][w];
+      tot_p += s_sum[1][w];
+    }
     __syncthreads();
     if (i < a.n) {
       s_tok[i] = (int32_t)(run_tok + off_t);
@@ -175,11 +199,18 @@ plan_step_kernel(const PlanArgs a) {
         if (blk >= 0 && blk < a.num_blocks) slot[j] = (int64_t)blk * a.bs + (pos - b * a.bs);
       }
     }
+    if (a.vec && t0 + kPlanGroup <= a.max_tokens) {
+      *reinterpret_cast<int4*>(a.ctx + t0) = make_int4(ctx[0], ctx[1], ctx[2], ctx[3]);
+      longlong2* out = reinterpret_cast<longlong2*>(a.slots + t0);
+      out[0] = make_longlong2(slot[0], slot[1]);
+      out[1] = make_longlong2(slot[2], slot[3]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < kPlanGroup; ++j) {
-      if (t0 + j < a.max_tokens) {
-        a.ctx[t0 + j] = ctx[j];
-        a.slots[t0 + j] = slot[j];
+      for (int j = 0; j < kPlanGroup; ++j) {
+        if (t0 + j < a.max_tokens) {
+          a.ctx[t0 + j] = ctx[j];
+          a.slots[t0 + j] = slot[j];
+        }
       }
     }
   }
@@ -234,21 +265,29 @@ extern "C" int clover_b200_plan_step(int32_t* free_stack, int32_t* free_top, int
   }
   PlanArgs a{free_stack, free_top, num_blocks, block_tables, table_stride, table_len, seq_lens,
              num_rows, rows, n_new, n_items, block_size, query_start_loc, ctx_lens, slot_mapping,
-             max_tokens, dev_status};
+             max_tokens,
+             ((reinterpret_cast<uintptr_t>(ctx_lens) | reinterpret_cast<uintptr_t>(slot_mapping)) & 15) == 0,
+             dev_status};
   const size_t smem = (size_t)(2 * (n_items + 1) + 3 * n_items + (num_rows + 31) / 32) * 4;
-  // One CTA covers a decode step; each further CTA takes 4 tokens per thread.
+  // One small CTA covers a decode step; admissions take up to 16 large ones.
+  const bool small = max_tokens <= 4 * kPlanSmall * kPlanGroup && n_items <= 4 * kPlanSmall;
+  const int threads = small ? kPlanSmall : kPlanLarge;
   int ctas = 1;
-  while (ctas < 8 && (int64_t)ctas * kPlanThreads * kPlanGroup < max_tokens) ctas *= 2;
-  if (smem > 48 * 1024) {
-    const int rc = check_cuda(cudaFuncSetAttribute(plan_step_kernel,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)smem),
+  while (!small && ctas < 16 && (int64_t)ctas * threads * kPlanGroup < max_tokens) ctas *= 2;
+  void (*kern)(PlanArgs) = small ? plan_step_kernel<kPlanSmall> : plan_step_kernel<kPlanLarge>;
+  if (smem > 40 * 1024) {
+    const int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                               "plan_step shared memory");
+    if (rc) return rc;
+  }
+  if (ctas > 8) {
+    const int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                              "plan_step cluster size");
     if (rc) return rc;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kPlanThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
@@ -258,5 +297,5 @@ extern "C" int clover_b200_plan_step(int32_t* free_stack, int32_t* free_top, int
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, plan_step_kernel, a), "plan_step launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "plan_step launch");
 }
