@@ -9,7 +9,7 @@ library, constructing a backend raises.
 """
 
 from .backend import B200AttentionBackend  # noqa: F401
-from .kv_cache import KVCacheManager, PagedKVPool  # noqa: F401
+from .kv_cache import DiffAttention, KVCacheManager, PagedKVPool  # noqa: F401
 from .head_groups import (build_head_groups, effective_group_count, group_ranges,  # noqa: F401
                           kv_head_shards, place_group, placement_rotation)
 from .sharded import HeadShardGroup  # noqa: F401
@@ -17,7 +17,7 @@ from ._lib import (CloverB200Error, attend_workspace_bytes, diff_decode, kv_appe
                    lib, lib_path, plan_step, scaled_decode)
 
 __all__ = [
-    "B200AttentionBackend", "KVCacheManager", "PagedKVPool", "HeadShardGroup",
+    "B200AttentionBackend", "KVCacheManager", "PagedKVPool", "DiffAttention", "HeadShardGroup",
     "CloverB200Error", "build_head_groups", "effective_group_count", "group_ranges",
     "kv_head_shards", "place_group", "placement_rotation", "lib", "lib_path",
     "plan_step", "kv_append_scaled", "scaled_decode", "diff_decode", "attend_workspace_bytes",

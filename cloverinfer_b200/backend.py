@@ -29,7 +29,14 @@ all-gather of the outputs.
 ``decode_batch`` is the tensor API for a step-batched engine
 (src/core/scheduler.py:980-1093): ``query [T, Hq, D]``, ``key/value [T, Hkv, D]``
 for ``T = sum(n_new)`` new tokens (causal among a sequence's new tokens),
-returning ``[T, Hq, D]`` on the GPU without a host sync.
+returning ``[T, Hq, D]`` on the GPU without a host sync.  ``begin_step`` plans a
+step once for all layers on the GPU, and ``decode_planned`` runs a layer of it.
+
+``kv_dtype=torch.int8`` (or ``torch.float8_e4m3fn`` with ``kv_scales=True``) keeps
+the cache in 8 bits with a scale per token and KV head; ``differential`` gives
+each layer's differential attention (``DiffAttention``: two softmax maps over the
+halves of head_dim, their difference normed).  Both run on every path above;
+sharded, their outputs go through NCCL.
 """
 
 from __future__ import annotations
@@ -45,7 +52,7 @@ import torch
 
 from . import _lib
 from .head_groups import local_inputs, select_kv_heads
-from .kv_cache import PagedKVPool, auto_partition, to_device_i32
+from .kv_cache import DiffAttention, PagedKVPool, auto_partition, to_device_i32
 
 
 _HOST_Q_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -65,6 +72,18 @@ class _Stats:
     items: int = 0
     tokens: int = 0
     kv_bytes_read: int = 0
+
+
+@dataclass
+class PlannedStep:
+    """A step planned by ``begin_step``: one for all layers."""
+    reqs: List[_Request]
+    n_new: List[int]
+    targets: List[int]
+    rows: torch.Tensor             # [B] table rows
+    query_start_loc: torch.Tensor  # [B + 1]
+    ctx_lens: torch.Tensor         # [T]
+    slots: torch.Tensor            # [T]
 
 
 class _FastPlan:
@@ -141,7 +160,8 @@ class B200AttentionBackend:
                  device=None, kv_cache_fraction: float = 0.5, partition_tokens: int = 0,
                  shard=None, check_status: bool = True, shuffle_seed: Optional[int] = None,
                  gather: str = "peer", max_rows_per_call: Optional[int] = None,
-                 cuda_graphs: bool = True, max_fast_plans: int = 8, **_unused) -> None:
+                 cuda_graphs: bool = True, max_fast_plans: int = 8, kv_scales: bool = False,
+                 differential: Optional[Sequence[DiffAttention]] = None, **_unused) -> None:
         self.device = torch.device(device) if device is not None else _default_device()
         if self.device.type != "cuda":
             raise RuntimeError("B200AttentionBackend requires a CUDA device (no CPU fallback)")
@@ -159,6 +179,9 @@ class B200AttentionBackend:
         self.shard = shard
         self.check_status = bool(check_status)
         self.shuffle_seed = shuffle_seed
+        self.kv_scales = bool(kv_scales)
+        self.differential = None if differential is None else list(differential)
+        self._diff: List[DiffAttention] = []  # this rank's heads, per layer
         if gather not in ("peer", "nccl"):
             raise ValueError("gather must be 'peer' or 'nccl'")
         self.gather_mode = gather
@@ -196,8 +219,17 @@ class B200AttentionBackend:
         if heads % hkv:
             raise ValueError(f"initial_kv has {heads} heads, not a multiple of num_kv_heads={hkv}")
         dt = self.kv_dtype or dtype
-        if dt not in (torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn):
+        if dt not in (torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.int8):
             raise TypeError(f"unsupported KV dtype {dt}")
+        if self.kv_scales and dt not in (torch.float8_e4m3fn, torch.int8):
+            raise TypeError(f"kv_scales needs an 8-bit cache, got {dt}")
+        if self.differential is not None:
+            if head_dim % 2:
+                raise ValueError(f"differential attention needs an even head_dim, got {head_dim}")
+            if len(self.differential) != num_layers:
+                raise ValueError(f"{len(self.differential)} differential layers for {num_layers} layers")
+            if dt == torch.float8_e4m3fn and not self.kv_scales:
+                raise TypeError("differential attention over float8_e4m3fn needs kv_scales=True")
         self.num_layers, self.num_kv_heads, self.head_dim, self.kv_dtype = num_layers, hkv, head_dim, dt
         self._kv_esz = torch.empty((), dtype=dt).element_size()
         if self.shard is not None:
@@ -207,14 +239,15 @@ class B200AttentionBackend:
         local = self.kv_range[1] - self.kv_range[0]
         nb = self.num_blocks
         esz = torch.empty((), dtype=dt).element_size()
-        per_block = 2 * num_layers * self.block_size * local * head_dim * esz
+        scaled = self.kv_scales or dt == torch.int8
+        per_block = 2 * num_layers * self.block_size * local * (head_dim * esz + (4 if scaled else 0))
         if nb is None:
             free, _ = torch.cuda.mem_get_info(self.device)
             nb = max(16, int(free * self.kv_cache_fraction) // per_block)
         width = min(nb, -(-self.max_seq_len // self.block_size) + 1)
         self.pool = PagedKVPool(nb, self.block_size, local, head_dim, num_layers=num_layers,
                                 dtype=dt, device=self.device, max_seqs=self.max_seqs,
-                                max_blocks_per_seq=width)
+                                max_blocks_per_seq=width, scaled=scaled)
         if self.shuffle_seed is not None:
             self.pool.shuffle_free_stack(self.shuffle_seed)
 
@@ -225,8 +258,31 @@ class B200AttentionBackend:
 
     def _local_kv(self, x: torch.Tensor) -> torch.Tensor:
         """[T, H, D] on device in the cache dtype, local KV heads only."""
-        return self._select_heads(x).to(device=self.device, dtype=self.kv_dtype,
+        return self._select_heads(x).to(device=self.device, dtype=self.pool.new_dtype(x.dtype),
                                         non_blocking=True).contiguous()
+
+    @property
+    def _own_attend(self) -> bool:
+        """Whether steps run on the scaled / differential decodes (which splits
+        and gathers of the plain one do not apply to)."""
+        return self.pool.scaled or self.differential is not None
+
+    def _q_dtypes(self):
+        """Query dtypes the decode takes as they are."""
+        return _HOST_Q_DTYPES if self.pool.scaled else (torch.float32, self.kv_dtype)
+
+    def _diff_layer(self, layer: int, num_q_heads: int) -> Optional[DiffAttention]:
+        """This rank's heads of a layer's differential attention, on this device."""
+        if self.differential is None:
+            return None
+        if not self._diff:
+            lo, hi = self.kv_range
+            group = num_q_heads // self.num_kv_heads
+            for d in self.differential:
+                if d.lam.numel() != num_q_heads:
+                    raise ValueError(f"differential lam has {d.lam.numel()} heads, queries {num_q_heads}")
+            self._diff = [d.heads(lo * group, hi * group, self.device) for d in self.differential]
+        return self._diff[layer]
 
     def _ingest(self, row: int, initial_kv, T: int) -> None:
         """Every layer's prefill K/V into the pool in one pass: this rank's
@@ -245,12 +301,13 @@ class B200AttentionBackend:
         ing = self._ingest_stream
         ing.wait_stream(cur)  # the blocks were reserved (and inputs made) on the decode stream
         on_host = not initial_kv[0]["key"].is_cuda
+        dtype = pool.new_dtype(initial_kv[0]["key"].dtype)
         with torch.cuda.stream(ing):
             shape = (L, 2, T, hl, self.head_dim)
             if on_host:
-                stage = torch.empty(shape, dtype=self.kv_dtype, pin_memory=True)
+                stage = torch.empty(shape, dtype=dtype, pin_memory=True)
             else:
-                stage = torch.empty(shape, dtype=self.kv_dtype, device=self.device)
+                stage = torch.empty(shape, dtype=dtype, device=self.device)
             for li, layer in enumerate(initial_kv):
                 for j, name in ((0, "key"), (1, "value")):
                     src = layer[name]
@@ -260,7 +317,7 @@ class B200AttentionBackend:
             dev = stage.to(self.device, non_blocking=True) if on_host else stage
             meta = to_device_i32([row, 0, 0, T], self.device)
             slots = pool.slots(meta[0:1], meta[1:2], meta[2:4], T)
-            _lib.kv_append_layers(pool.k, pool.v, dev[:, 0], dev[:, 1], slots, pool.status)
+            pool.append_layers(dev[:, 0], dev[:, 1], slots)
             ev = torch.cuda.Event()
             ev.record(ing)
         self._pending_ingest.append(ev)
@@ -469,6 +526,8 @@ class B200AttentionBackend:
     def _split(self, targets, n_new) -> int:
         """partition_tokens for this call: the caller's, or the host's choice
         from the batch's contexts (kv_cache.auto_partition)."""
+        if self._own_attend:
+            return 0
         if self.partition_tokens:
             return self.partition_tokens
         sharded = self.shard is not None and self.shard.world > 1
@@ -496,17 +555,22 @@ class B200AttentionBackend:
         group = plan.q.shape[1] // self.num_kv_heads
         lo, hi = self.kv_range
         q = plan.q if q_local_is_whole(lo, hi, self.num_kv_heads) else plan.q[:, lo * group:hi * group]
-        if q.dtype not in (torch.float32, self.kv_dtype) or q.stride(2) != 1 or q.stride(1) != self.head_dim:
+        if q.dtype not in self._q_dtypes() or q.stride(2) != 1 or q.stride(1) != self.head_dim:
             return None
         peer = self._peer_for(q) if sharded else None
         if sharded and peer is None:
             return None  # NCCL gather: stays eager
         B = q.shape[0]
-        if plan.k.shape[1] != self.num_kv_heads or plan.k.dtype != self.kv_dtype:
+        if plan.k.shape[1] != self.num_kv_heads or plan.k.dtype != pool.new_dtype(plan.k.dtype):
             return None  # K/V need a copy (expanded heads, other dtype): stays eager
         k_loc, v_loc = plan.k[:, lo:hi], plan.v[:, lo:hi]  # token stride spans all heads
         n_seqs = B
-        if peer is not None:
+        diff = self._diff_layer(layer, plan.q.shape[1])
+        if self._own_attend:
+            nbytes = _lib.attend_workspace_bytes(n_seqs, B, 1, bucket, q.shape[1], pool.num_kv_heads,
+                                                 self.head_dim, pool.block_size, pool.dtype, q.dtype,
+                                                 diff is not None)
+        elif peer is not None:
             nbytes = _lib.decode_gather_workspace_bytes(n_seqs, B, 1, bucket, q.shape[1], pool.num_kv_heads,
                                                         self.head_dim, pool.block_size, pool.dtype,
                                                         q.dtype, pt)
@@ -531,7 +595,10 @@ class B200AttentionBackend:
                 # (all-gathered) output and its status bits into the plan's
                 # result buffer; the caller copies that back after the launch.
                 plan.dev.copy_(plan.host, non_blocking=True)
-                if peer is not None:
+                if self._own_attend:
+                    pool.attend(layer, q, plan.offs_d, plan.ctx, plan.rows, 1, bucket, scale, k_new=k_loc,
+                                v_new=v_loc, diff=diff, out=out_dev, workspace=ws, status=plan.status_dev)
+                elif peer is not None:
                     _lib.decode_step_gather(q, pool.k[layer], pool.v[layer], k_loc, v_loc, pool.tables,
                                             plan.offs_d, plan.ctx, peer, max_queries_per_seq=1,
                                             max_ctx_len=bucket, score_scale=scale, seq_rows=plan.rows,
@@ -605,6 +672,75 @@ class B200AttentionBackend:
         # the fused gather's buffer is rewritten by the next call
         return res.clone() if self._peer is not None and res.data_ptr() == self._peer.out.data_ptr() else res
 
+    def begin_step(self, request_ids: Sequence[str], n_new: Optional[Sequence[int]] = None) -> PlannedStep:
+        """Plan a step of ``n_new[b]`` new tokens per request (default 1) once for all
+        layers: one small copy of rows and lengths, and one launch that grows the block
+        tables and lays out slots, contexts and query offsets on the GPU
+        (``clover_b200_plan_step``).  Run it with ``decode_planned``, every layer once.
+        Raises before any state changes, like ``decode_batch``; a request's layers must
+        hold the same number of tokens."""
+        pool = self.pool
+        if pool is None:
+            raise KeyError("no request has been initialised")
+        n_new = [1] * len(request_ids) if n_new is None else [int(n) for n in n_new]
+        if len(n_new) != len(request_ids) or any(n < 0 for n in n_new):
+            raise ValueError(f"n_new must be {len(request_ids)} counts, none negative")
+        reqs = []
+        for r in request_ids:
+            if r not in self._reqs:
+                raise KeyError(f"Unknown request {r}")
+            reqs.append(self._reqs[r])
+            if len(set(reqs[-1].layer_len)) != 1:
+                raise RuntimeError(f"request {r} is inside a step: its layers hold different lengths")
+        rows, held = [r.row for r in reqs], [r.layer_len[0] for r in reqs]
+        if len(set(rows)) != len(rows):
+            raise ValueError("begin_step: duplicate requests in one step")
+        targets = [h + n for h, n in zip(held, n_new)]
+        need = pool.demand(rows, targets)
+        if need > pool.free_count:
+            raise RuntimeError("OOM during append")
+        if self._pending_ingest:
+            self._await_ingest()
+        B = len(rows)
+        meta = to_device_i32(rows + held + n_new, self.device)
+        pool.set_seq_lens(meta[:B], meta[B:2 * B])
+        p = pool.plan_step(meta[:B], meta[2 * B:], sum(n_new))
+        for r, t, n in zip(rows, targets, n_new):
+            if n:
+                pool.row_blocks[r] = max(pool.row_blocks[r], pool.blocks_for(t))
+        pool.free_count -= need
+        return PlannedStep(reqs, n_new, targets, p.rows, p.query_start_loc, p.ctx_lens, p.slots)
+
+    def decode_planned(self, step: PlannedStep, layer_idx: int, query: torch.Tensor, key: torch.Tensor,
+                       value: torch.Tensor, score_scale: float = 1.0,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One layer of a planned step: append its new K/V and attend.  Tensors, result and
+        ``out`` as in ``decode_batch``."""
+        if not 0 <= layer_idx < self.num_layers:
+            raise IndexError(f"layer_idx {layer_idx} out of range [0, {self.num_layers})")
+        T = sum(step.n_new)
+        hq, d = int(query.shape[1]), int(query.shape[2])
+        if query.shape[0] != T or key.shape[0] != T or value.shape[0] != T:
+            raise ValueError(f"expected {T} new tokens, got q {tuple(query.shape)} k {tuple(key.shape)}")
+        if hq % self.num_kv_heads or d != self.head_dim:
+            raise ValueError(f"query heads x dim {hq} x {d} do not fit {self.num_kv_heads} KV heads x {self.head_dim}")
+        for r, t, n in zip(step.reqs, step.targets, step.n_new):
+            if r.layer_len[layer_idx] != t - n:
+                raise RuntimeError(f"layer {layer_idx} of the step has run already, or its requests went on")
+        if self._pending_ingest:
+            self._await_ingest()
+        dst = None if out is None else self._consumer_view(out, T, hq)
+        query, key, value = (x if x.is_cuda else x.to(self.device, non_blocking=True) for x in (query, key, value))
+        if T == 0:
+            return torch.empty_like(query) if dst is None else dst
+        res = self._launch(step.reqs, layer_idx, step.n_new, step.targets, query, key, value, step.rows,
+                           step.query_start_loc, step.ctx_lens, score_scale, dst=dst)
+        if dst is not None:
+            if res.data_ptr() != dst.data_ptr():
+                dst.copy_(res)
+            return dst
+        return res.clone() if self._peer is not None and res.data_ptr() == self._peer.out.data_ptr() else res
+
     def _h2d(self, x: torch.Tensor) -> torch.Tensor:
         """A host tensor on this backend's device, copied asynchronously: a
         view of some heads (rows of contiguous values at a wider stride) goes
@@ -671,20 +807,27 @@ class B200AttentionBackend:
         group = hq // self.num_kv_heads
         lo, hi = self.kv_range
         q = query.to(self.device, non_blocking=True)
-        if q.dtype not in (torch.float32, self.kv_dtype):
+        if q.dtype not in self._q_dtypes():
             q = q.float()
         if not local and (lo, hi) != (0, self.num_kv_heads):
             q = q[:, lo * group:hi * group]
         if q.stride(2) != 1 or q.stride(1) != self.head_dim:
             q = q.contiguous()
         if local:
-            k_loc = key.to(dtype=self.kv_dtype).contiguous()
-            v_loc = value.to(dtype=self.kv_dtype).contiguous()
+            k_loc = key.to(dtype=pool.new_dtype(key.dtype)).contiguous()
+            v_loc = value.to(dtype=pool.new_dtype(value.dtype)).contiguous()
         else:
             k_loc, v_loc = self._local_kv(key), self._local_kv(value)
         sharded = self.shard is not None and self.shard.world > 1
         peer = self._peer_for(q) if sharded else None
-        if peer is not None:
+        if self._own_attend:
+            if k_loc.dtype != v_loc.dtype:
+                k_loc, v_loc = k_loc.float(), v_loc.float()
+            direct = dst is not None and not sharded and dst.dtype == q.dtype
+            out = pool.attend(layer_idx, q, offs_d, ctx_d, rows_d, max(n_new), max(targets), score_scale,
+                              k_new=k_loc, v_new=v_loc, diff=self._diff_layer(layer_idx, hq),
+                              out=dst if direct else None)
+        elif peer is not None:
             # fused append + decode + reduce with the all-gather over NVLink
             out = pool.decode_step_gather(layer_idx, q, k_loc, v_loc, offs_d, ctx_d, rows_d,
                                           max(n_new), max(targets), score_scale, peer,
@@ -719,11 +862,12 @@ class B200AttentionBackend:
         st.batches += 1
         st.items += len(reqs)
         st.tokens += len(reqs) if n_new is None else sum(n_new)
-        st.kv_bytes_read += sum(targets) * (hi - lo) * self.head_dim * 2 * self._kv_esz
+        st.kv_bytes_read += sum(targets) * (hi - lo) * 2 * (self.head_dim * self._kv_esz
+                                                            + (4 if self.pool.scaled else 0))
 
     def _peer_for(self, q: torch.Tensor):
         """The fused-gather buffers for this call's shape, or None (NCCL)."""
-        if self.gather_mode != "peer" or q.shape[0] > self.max_rows_per_call:
+        if self.gather_mode != "peer" or q.shape[0] > self.max_rows_per_call or self._own_attend:
             return None
         if self.num_kv_heads % self.shard.world:
             return None  # uneven shards: NCCL gather pads them
@@ -755,7 +899,8 @@ class B200AttentionBackend:
             info.update({
                 "num_layers": self.num_layers, "num_kv_heads": self.num_kv_heads,
                 "kv_heads_local": list(self.kv_range), "head_dim": self.head_dim,
-                "kv_dtype": str(self.kv_dtype), "block_size": pool.block_size,
+                "kv_dtype": str(self.kv_dtype), "kv_scaled": pool.scaled,
+                "differential": self.differential is not None, "block_size": pool.block_size,
                 "num_blocks": pool.num_blocks, "free_blocks": pool.free_count,
                 "kv_cache_bytes": 2 * pool.k.numel() * pool.k.element_size(),
             })

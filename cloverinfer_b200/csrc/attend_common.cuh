@@ -385,10 +385,10 @@ __device__ __forceinline__ void attend_record(const AttendArgs& a, const AttendS
 __device__ __forceinline__ float diff_value(float o1, float o2, float lam) { return fmaf(-lam, o2, o1); }
 
 // Host side (paged_attend_mma.cu): the tensor-core kernel for these types and
-// shape; cols 8 or 16.  a == null only reports its most CTAs and the workers of
-// one.
+// shape; cols 8 or 16.  a == null only reports the workers of a CTA (one CTA per
+// SM).
 bool attend_mma_supported(int kv_dtype, int q_dtype, int D, int bs);
 int attend_mma_unit_log2(int kv_dtype, int D);
-int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid, int* rings);
+int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* rings);
 
 }  // namespace clover

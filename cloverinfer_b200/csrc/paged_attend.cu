@@ -455,7 +455,7 @@ static int generic_grid(int sms) {
     int n = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attend_generic_kernel<KT, EPL, NC>,
                                                       kAttendThreads, 0) != cudaSuccess || n < 1)
-      n = 1;
+      return sms;
     cached = n > kAttendMaxPerSm / kAttendWarps ? kAttendMaxPerSm / kAttendWarps : n;
   }
   return cached * sms;
@@ -546,8 +546,8 @@ static int attend_shape(int n_seqs, int n_rows, int max_q, int max_ctx, int hq, 
   // Short contexts: a segment is at most two ranges' least work; splitting it
   // would cost the second launch more than it gains.
   p->whole = units <= 2 * least;
-  int grid = 0, rings = kAttendWarps;
-  const int rc = p->mma ? attend_mma(kv_dtype, q_dtype, p->cols, nullptr, D, nullptr, &grid, &rings)
+  int grid = p->sms, rings = kAttendWarps;
+  const int rc = p->mma ? attend_mma(kv_dtype, q_dtype, p->cols, nullptr, D, nullptr, &rings)
                         : attend_generic(kv_dtype, D, p->cols, nullptr, nullptr, p->sms, &grid);
   if (rc) return rc;
   const int64_t segs = (int64_t)n_seqs * hkv * chunks;
@@ -672,7 +672,7 @@ static int attend_impl(const char* what, void* out, int64_t out_row_stride, cons
     rc = check_cuda(cudaGetLastError(), "attend_append launch");
     if (rc) return rc;
   }
-  rc = sh.mma ? attend_mma(kv_dtype, q_dtype, sh.cols, &a, head_dim, s, nullptr, nullptr)
+  rc = sh.mma ? attend_mma(kv_dtype, q_dtype, sh.cols, &a, head_dim, s, nullptr)
               : attend_generic(kv_dtype, head_dim, sh.cols, &a, s, sh.sms, nullptr);
   if (rc || sh.whole) return rc;
   const cudaError_t e = maps == 2 ? launch_join<2>(a, sh.sms, s) : launch_join<1>(a, sh.sms, s);

@@ -917,29 +917,24 @@ static int attend_tmap(const void* ptr, int esz, int D, int H, int64_t slots, CU
 }
 
 template <int KV, bool QF32, int D, int CW>
-static int mma_launch(const AttendArgs* a, cudaStream_t s, int* grid, int* rings) {
+static int mma_launch(const AttendArgs* a, cudaStream_t s, int* rings) {
   using G = AttendGeom<KV, QF32, D, CW>;
+  if (a == nullptr) {
+    *rings = G::kRings;
+    return CLOVER_B200_OK;
+  }
   auto kern = attend_mma_kernel<KV, QF32, D, CW>;
-  static int sms[64] = {0};
+  static uint64_t configured = 0;  // one bit per device ordinal
   int dev = 0;
   int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   if (rc) return rc;
-  if (dev >= 64) return set_error(CLOVER_B200_ERR_UNSUPPORTED, "attend: device ordinal %d", dev);
   {
     std::lock_guard<std::mutex> lock(g_attend_mu);
-    if (sms[dev] == 0) {
+    if (dev >= 64 || !(configured >> dev & 1)) {
       rc = set_smem(kern, G::kSmem);
       if (rc) return rc;
-      int m = 0;
-      rc = check_cuda(cudaDeviceGetAttribute(&m, cudaDevAttrMultiProcessorCount, dev), "attend SMs");
-      if (rc) return rc;
-      sms[dev] = m;
+      if (dev < 64) configured |= 1ull << dev;
     }
-  }
-  if (a == nullptr) {
-    *grid = sms[dev];
-    *rings = G::kRings;
-    return CLOVER_B200_OK;
   }
   CUtensorMap tk, tv;
   rc = attend_tmap(a->kc, G::kEsz, D, a->hkv, a->num_blocks * a->bs, &tk);
@@ -951,12 +946,12 @@ static int mma_launch(const AttendArgs* a, cudaStream_t s, int* grid, int* rings
 }
 
 template <int KV, bool QF32>
-static int mma_shape(int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid, int* rings) {
+static int mma_shape(int cols, const AttendArgs* a, int D, cudaStream_t s, int* rings) {
   const bool two = cols > kMmaCols;
   switch (D) {
-    case 64: return two ? mma_launch<KV, QF32, 64, 2>(a, s, grid, rings) : mma_launch<KV, QF32, 64, 1>(a, s, grid, rings);
-    case 128: return two ? mma_launch<KV, QF32, 128, 2>(a, s, grid, rings) : mma_launch<KV, QF32, 128, 1>(a, s, grid, rings);
-    default: return two ? mma_launch<KV, QF32, 256, 2>(a, s, grid, rings) : mma_launch<KV, QF32, 256, 1>(a, s, grid, rings);
+    case 64: return two ? mma_launch<KV, QF32, 64, 2>(a, s, rings) : mma_launch<KV, QF32, 64, 1>(a, s, rings);
+    case 128: return two ? mma_launch<KV, QF32, 128, 2>(a, s, rings) : mma_launch<KV, QF32, 128, 1>(a, s, rings);
+    default: return two ? mma_launch<KV, QF32, 256, 2>(a, s, rings) : mma_launch<KV, QF32, 256, 1>(a, s, rings);
   }
 }
 
@@ -969,13 +964,13 @@ int attend_mma_unit_log2(int kv_dtype, int D) {
   return D * (eight ? 1 : 2) <= 128 ? 5 : 4;
 }
 
-int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* grid, int* rings) {
+int attend_mma(int kv_dtype, int q_dtype, int cols, const AttendArgs* a, int D, cudaStream_t s, int* rings) {
   const bool f32 = q_dtype == CLOVER_B200_F32;
   switch (kv_dtype) {
-    case CLOVER_B200_BF16: return f32 ? mma_shape<KV_BF16, true>(cols, a, D, s, grid, rings) : mma_shape<KV_BF16, false>(cols, a, D, s, grid, rings);
-    case CLOVER_B200_F16: return f32 ? mma_shape<KV_F16, true>(cols, a, D, s, grid, rings) : mma_shape<KV_F16, false>(cols, a, D, s, grid, rings);
-    case CLOVER_B200_INT8: return f32 ? mma_shape<KV_I8, true>(cols, a, D, s, grid, rings) : mma_shape<KV_I8, false>(cols, a, D, s, grid, rings);
-    default: return f32 ? mma_shape<KV_E4M3, true>(cols, a, D, s, grid, rings) : mma_shape<KV_E4M3, false>(cols, a, D, s, grid, rings);
+    case CLOVER_B200_BF16: return f32 ? mma_shape<KV_BF16, true>(cols, a, D, s, rings) : mma_shape<KV_BF16, false>(cols, a, D, s, rings);
+    case CLOVER_B200_F16: return f32 ? mma_shape<KV_F16, true>(cols, a, D, s, rings) : mma_shape<KV_F16, false>(cols, a, D, s, rings);
+    case CLOVER_B200_INT8: return f32 ? mma_shape<KV_I8, true>(cols, a, D, s, rings) : mma_shape<KV_I8, false>(cols, a, D, s, rings);
+    default: return f32 ? mma_shape<KV_E4M3, true>(cols, a, D, s, rings) : mma_shape<KV_E4M3, false>(cols, a, D, s, rings);
   }
 }
 

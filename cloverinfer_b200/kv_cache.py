@@ -15,6 +15,14 @@ The host keeps only counters (free blocks, blocks per row) so it can raise the
 upstream errors (``RuntimeError`` on exhaustion, :64-65, :108-109) before any
 kernel runs; block ids never leave the GPU on the hot path.
 
+An 8-bit pool (``dtype=torch.int8``, or ``torch.float8_e4m3fn`` with
+``scaled=True``) also holds one fp32 scale per (token, KV head) for K and for V,
+``k_scale``/``v_scale`` ``[layers, num_blocks, num_kv_heads, block_size]``; new
+tokens come in f32, f16 or bf16 and are quantised by the append.
+
+``plan_step`` plans a step from lengths on the GPU (``seq_lens``), with no host
+bookkeeping: a captured plan + append + decode can be replayed step after step.
+
 ``KVCacheManager`` is the drop-in for the upstream class of the same name:
 same constructor, methods, return values and errors, backed by the pool.
 """
@@ -22,6 +30,7 @@ same constructor, methods, return values and errors, backed by the pool.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -51,10 +60,56 @@ def auto_partition(contexts: Sequence[int], max_q: int, sharded: bool = False) -
     return _lib.PARTITION_BALANCED if longest * n >= 1.25 * sum(contexts) and longest > 0 else 0
 
 
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+@dataclass(frozen=True)
+class DiffAttention:
+    """One layer's differential attention: per query head ``lam`` (float32 [Hq]), and
+    the norm of its output (``norm_weight`` float32 [head_dim] or None, ``eps``,
+    ``out_scale``): out = norm(softmax_1 V - lam * softmax_2 V)."""
+    lam: torch.Tensor
+    norm_weight: Optional[torch.Tensor] = None
+    eps: float = 1e-5
+    out_scale: float = 1.0
+
+    @classmethod
+    def from_vectors(cls, q1: torch.Tensor, k1: torch.Tensor, q2: torch.Tensor, k2: torch.Tensor,
+                     lambda_init: float, num_heads: int, norm_weight: Optional[torch.Tensor] = None,
+                     eps: float = 1e-5) -> "DiffAttention":
+        """From the learned vectors ([d], or [num_heads, d]): lam = exp(q1 . k1) -
+        exp(q2 . k2) + lambda_init, computed once in 64 bits; the norm's output is
+        scaled by 1 - lambda_init."""
+        lam = (q1.double() * k1.double()).sum(-1).exp() - (q2.double() * k2.double()).sum(-1).exp() + lambda_init
+        return cls(lam.float().expand(num_heads).contiguous(), norm_weight, eps, 1.0 - float(lambda_init))
+
+    def heads(self, lo: int, hi: int, device) -> "DiffAttention":
+        """The query heads [lo, hi) on ``device`` (this object if that is all of them, there)."""
+        device = torch.device(device)
+        if (lo, hi) == (0, self.lam.numel()) and self.lam.device == device:
+            return self
+        w = None if self.norm_weight is None else self.norm_weight.to(device=device, dtype=torch.float32).contiguous()
+        return DiffAttention(self.lam[lo:hi].to(device=device, dtype=torch.float32).contiguous(), w, self.eps,
+                             self.out_scale)
+
+
+@dataclass
+class StepPlan:
+    """What :meth:`PagedKVPool.plan_step` made of one step, on the GPU."""
+    rows: torch.Tensor             # [B] table rows
+    query_start_loc: torch.Tensor  # [B + 1]
+    ctx_lens: torch.Tensor         # [max_tokens]
+    slots: torch.Tensor            # [max_tokens], -1 past the last token
+
+
 class PagedKVPool:
     def __init__(self, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int, *,
                  num_layers: int = 1, dtype: torch.dtype = torch.bfloat16,
-                 device="cuda", max_seqs: int = 256, max_blocks_per_seq: Optional[int] = None) -> None:
+                 device="cuda", max_seqs: int = 256, max_blocks_per_seq: Optional[int] = None,
+                 scaled: Optional[bool] = None) -> None:
+        self.scaled = dtype == torch.int8 if scaled is None else bool(scaled)
+        if self.scaled != (dtype == torch.int8) and dtype != torch.float8_e4m3fn:
+            raise TypeError(f"PagedKVPool: a {dtype} cache {'has no' if self.scaled else 'needs'} scales")
         if num_blocks <= 0 or block_size <= 0 or num_kv_heads <= 0 or head_dim <= 0:
             raise ValueError("PagedKVPool: sizes must be positive")
         self.device = torch.device(device)
@@ -74,10 +129,17 @@ class PagedKVPool:
         dev = self.device
         self.k = torch.zeros(shape, dtype=dtype, device=dev)
         self.v = torch.zeros(shape, dtype=dtype, device=dev)
+        self.k_scale = self.v_scale = None
+        if self.scaled:
+            sshape = (self.num_layers, self.num_blocks, self.num_kv_heads, self.block_size)
+            self.k_scale = torch.zeros(sshape, dtype=torch.float32, device=dev)
+            self.v_scale = torch.zeros(sshape, dtype=torch.float32, device=dev)
         self.free_stack = torch.arange(self.num_blocks, dtype=torch.int32, device=dev)
         self.free_top = torch.tensor([self.num_blocks], dtype=torch.int32, device=dev)
         self.tables = torch.full((self.max_seqs, self.max_blocks_per_seq), -1, dtype=torch.int32, device=dev)
         self.table_len = torch.zeros(self.max_seqs, dtype=torch.int32, device=dev)
+        # tokens held per row, for plan_step (the host paths do not use it)
+        self.seq_lens = torch.zeros(self.max_seqs, dtype=torch.int32, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         # host mirror: counters only
         self.free_count = self.num_blocks
@@ -161,9 +223,80 @@ class PagedKVPool:
                            self.num_blocks, out, self.status)
         return out
 
+    # ------------------------------------------------------------ plan on the GPU
+    def set_seq_lens(self, rows: torch.Tensor, lens: torch.Tensor) -> None:
+        """Tell ``plan_step`` how many tokens rows hold (device int32 tensors)."""
+        self.seq_lens.index_copy_(0, rows.long(), lens)
+
+    def plan_step(self, rows: torch.Tensor, n_new: torch.Tensor, max_tokens: int) -> StepPlan:
+        """Plan one step from ``seq_lens`` on the GPU: grow the tables of ``rows`` (device
+        int32; negative: padding) for ``n_new`` (device int32) more tokens each, at most
+        ``max_tokens`` in all, and advance ``seq_lens``.  No host sync and no host
+        bookkeeping: ``refresh_host`` brings the host counters in line before host paths
+        (``reserve``, ``release``, ...) touch the pool again.  A step that does not fit
+        changes nothing, plans nothing and raises a bit in ``status``.  With padding or
+        zero counts inside the batch, pass the decodes ``max_q`` >= 2 unless they are the
+        scaled or differential ones (with max_q = 1 the others take row b for sequence b)."""
+        dev = self.device
+        qsl = torch.empty(rows.numel() + 1, dtype=torch.int32, device=dev)
+        ctx = torch.empty(int(max_tokens), dtype=torch.int32, device=dev)
+        slots = torch.empty(int(max_tokens), dtype=torch.int64, device=dev)
+        _lib.plan_step(self.free_stack, self.free_top, self.tables, self.table_len, self.seq_lens, rows, n_new,
+                       self.block_size, qsl, ctx, slots, self.status)
+        return StepPlan(rows, qsl, ctx, slots)
+
+    def refresh_host(self) -> None:
+        """Host counters from the device state (synchronises)."""
+        self.free_count = int(self.free_top.item())
+        self.row_blocks = self.table_len.tolist()
+
     # ------------------------------------------------------------ data path
+    def new_dtype(self, dtype: torch.dtype) -> torch.dtype:
+        """The dtype new K/V of ``dtype`` are handed to the append in: the cache's, or
+        for a scaled cache any float type as it is."""
+        if not self.scaled:
+            return self.dtype
+        return dtype if dtype in _FLOATS else torch.float32
+
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, slots: torch.Tensor) -> None:
-        _lib.kv_append(self.k[layer], self.v[layer], k_new, v_new, slots, self.status)
+        if self.scaled:
+            _lib.kv_append_scaled(self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], k_new,
+                                  v_new, slots, self.status)
+        else:
+            _lib.kv_append(self.k[layer], self.v[layer], k_new, v_new, slots, self.status)
+
+    def append_layers(self, k_new: torch.Tensor, v_new: torch.Tensor, slots: torch.Tensor) -> None:
+        """Every layer's new tokens [L, n, H, D] in one launch."""
+        if self.scaled:
+            _lib.kv_append_scaled(self.k, self.v, self.k_scale, self.v_scale, k_new, v_new, slots, self.status)
+        else:
+            _lib.kv_append_layers(self.k, self.v, k_new, v_new, slots, self.status)
+
+    def scales(self, layer: int):
+        """(k_scale, v_scale) of a layer, (None, None) without scales."""
+        return (self.k_scale[layer], self.v_scale[layer]) if self.scaled else (None, None)
+
+    def attend(self, layer: int, q: torch.Tensor, query_start_loc: torch.Tensor, ctx_lens: torch.Tensor,
+               seq_rows: Optional[torch.Tensor], max_q: int, max_ctx: int, score_scale: float, *,
+               k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None,
+               diff: Optional[DiffAttention] = None, out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The decodes over a scaled cache, and differential ones (``diff``) over any:
+        append k_new/v_new at ctx - 1 if given, then attend."""
+        if out is None:
+            out = torch.empty_like(q)
+        ks, vs = self.scales(layer)
+        kw = dict(max_queries_per_seq=max_q, max_ctx_len=max_ctx, score_scale=score_scale, k_new=k_new,
+                  v_new=v_new, seq_rows=seq_rows, workspace=workspace,
+                  status=self.status if status is None else status)
+        if diff is not None:
+            _lib.diff_decode(out, q, self.k[layer], self.v[layer], diff.lam, self.tables, query_start_loc,
+                             ctx_lens, norm_weight=diff.norm_weight, eps=diff.eps, out_scale=diff.out_scale,
+                             k_scales=ks, v_scales=vs, **kw)
+        else:
+            _lib.scaled_decode(out, q, self.k[layer], self.v[layer], ks, vs, self.tables, query_start_loc,
+                               ctx_lens, **kw)
+        return out
 
     def workspace(self, nbytes: int) -> Optional[torch.Tensor]:
         """A reusable device workspace of at least ``nbytes`` (grown, never shrunk)."""
@@ -176,6 +309,8 @@ class PagedKVPool:
     def decode(self, layer: int, q: torch.Tensor, query_start_loc: torch.Tensor, ctx_lens: torch.Tensor,
                seq_rows: Optional[torch.Tensor], max_q: int, max_ctx: int, score_scale: float,
                out: Optional[torch.Tensor] = None, partition_tokens: int = 0) -> torch.Tensor:
+        if self.scaled:  # (splits by itself: partition_tokens does not apply)
+            return self.attend(layer, q, query_start_loc, ctx_lens, seq_rows, max_q, max_ctx, score_scale, out=out)
         if out is None:
             out = torch.empty_like(q)
         n_seqs = query_start_loc.numel() - 1
@@ -196,6 +331,9 @@ class PagedKVPool:
                     check: bool = True) -> torch.Tensor:
         """Append every query row's new token at ctx - 1 and attend (one fused
         launch for a plain decode step).  Capacity must be reserved first."""
+        if self.scaled:
+            return self.attend(layer, q, query_start_loc, ctx_lens, seq_rows, max_q, max_ctx, score_scale,
+                               k_new=k_new, v_new=v_new, out=out)
         if out is None:
             out = torch.empty_like(q)
         n_seqs = query_start_loc.numel() - 1
@@ -217,7 +355,9 @@ class PagedKVPool:
         """decode_step for a head-sharded group: the all-gathered output of
         every rank lands in ``out`` ([rows, Hq_total, D] view of a consumer
         buffer, any f32/f16/bf16) or in ``gather.out`` (returned view, valid
-        until the next call)."""
+        until the next call).  Not for scaled caches."""
+        if self.scaled:
+            raise TypeError("decode_step_gather: a scaled cache has no fused gather")
         n_seqs = query_start_loc.numel() - 1
         nbytes = _lib.decode_gather_workspace_bytes(n_seqs, q.shape[0], max_q, max_ctx, q.shape[1],
                                                     self.num_kv_heads, self.head_dim,
@@ -243,7 +383,8 @@ class PagedKVPool:
         """Raise the RuntimeError that names the CLOVER_B200_DEV_* bits of ``code``."""
         names = [n for n, bit in [("bad slot", _lib.DEV_BAD_SLOT), ("bad block id", _lib.DEV_BAD_BLOCK),
                                   ("table full", _lib.DEV_TABLE_FULL), ("out of blocks", _lib.DEV_OOM),
-                                  ("wait timeout", _lib.DEV_TIMEOUT), ("context > max_ctx_len", _lib.DEV_CTX_RANGE)]
+                                  ("wait timeout", _lib.DEV_TIMEOUT), ("context > max_ctx_len", _lib.DEV_CTX_RANGE),
+                                  ("bad step plan", _lib.DEV_BAD_PLAN)]
                  if code & bit]
         raise RuntimeError(f"libclover_b200 device status 0x{code:x}: {', '.join(names)}")
 
@@ -309,8 +450,9 @@ class KVCacheManager:
             pd = to_device_i32([0], dev)
             od = to_device_i32([0, n], dev)
             slots = self.pool.slots(rd, pd, od, n)
-            k = k_data.to(device=dev, dtype=self.dtype).contiguous()
-            v = v_data.to(device=dev, dtype=self.dtype).contiguous()
+            dt = self.pool.new_dtype(k_data.dtype)
+            k = k_data.to(device=dev, dtype=dt).contiguous()
+            v = v_data.to(device=dev, dtype=dt).contiguous()
             self.pool.append(0, k, v, slots)
         self.context_lens[request_id] = n
 
@@ -336,8 +478,9 @@ class KVCacheManager:
         row = self._rows[request_id]
         slots = self.pool.slots(to_device_i32([row], dev), to_device_i32([pos], dev),
                                 to_device_i32([0, 1], dev), 1)
-        self.pool.append(0, k.to(device=dev, dtype=self.dtype).reshape(1, self.num_heads, self.head_dim).contiguous(),
-                         v.to(device=dev, dtype=self.dtype).reshape(1, self.num_heads, self.head_dim).contiguous(),
+        dt = self.pool.new_dtype(k.dtype)
+        self.pool.append(0, k.to(device=dev, dtype=dt).reshape(1, self.num_heads, self.head_dim).contiguous(),
+                         v.to(device=dev, dtype=dt).reshape(1, self.num_heads, self.head_dim).contiguous(),
                          slots)
 
     # memory_manager.py:134-143
