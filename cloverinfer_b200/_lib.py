@@ -339,13 +339,18 @@ def _one_device(what, *ts) -> int:
     return dev
 
 
+# the current stream's handle without a Stream object (over 1 us of a small call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _call_on(dev: int, fn, *args) -> int:
     """Call a launching entry point with its tensors' device current and its
     current stream as the last argument."""
     if dev == torch.cuda.current_device():
-        return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        return fn(*args, _raw_stream(dev))
     with torch.cuda.device(dev):
-        return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        return fn(*args, _raw_stream(dev))
 
 
 def _index_i32(what, *ts) -> None:

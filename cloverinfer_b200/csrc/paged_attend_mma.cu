@@ -101,6 +101,15 @@ __device__ __forceinline__ uint32_t attend_swz(int r, int c) {
   return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
+// attend_swz(r, c + 2 i) from the address of attend_swz(r, c), c in {0, 1}: the
+// swizzle is an exclusive or of the chunk's low bits, so an even step is one
+// instruction (tile rows start on a multiple of the swizzled row).
+template <int SWZ, int TOK>
+__device__ __forceinline__ uint32_t attend_swz_step(uint32_t at, int i) {
+  constexpr int kGroup = SWZ / 16;  // chunks of a swizzled row
+  return (at ^ (uint32_t)((2 * i % kGroup) << 4)) + (uint32_t)(2 * i / kGroup * TOK * SWZ);
+}
+
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t d;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
@@ -305,20 +314,23 @@ template <int KV, int SWZ, int TOK>
 struct VFrag {
   static constexpr int kPer = KV >= KV_I8 ? 2 : 1;
   uint32_t a[kPer][4];
-  __device__ __forceinline__ void load(uint32_t vs, int i, int lane) {
+  // This lane's row and chunk of the first load.
+  __device__ __forceinline__ static uint32_t first(int lane) {
     const int grp = lane >> 3;
+    return KV >= KV_I8 ? attend_swz<SWZ, TOK>((lane & 7) + (grp & 1) * 8, grp >> 1)
+                       : attend_swz<SWZ, TOK>((lane & 7) + (grp >> 1) * 8, grp & 1);
+  }
+  __device__ __forceinline__ void load(uint32_t va, int i) {
     if (KV >= KV_I8) {
-      const int r = (lane & 7) + (grp & 1) * 8;
       uint32_t x[4];
-      ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp >> 1)), x[0], x[1], x[2], x[3]);
+      ldsm_x4_trans(attend_swz_step<SWZ, TOK>(va, i), x[0], x[1], x[2], x[3]);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
         codes_to_f16<KV>(x[2 * k], a[k][0], a[k][1]);
         codes_to_f16<KV>(x[2 * k + 1], a[k][2], a[k][3]);
       }
     } else {
-      const int r = (lane & 7) + (grp >> 1) * 8;
-      ldsm_x4_trans(vs + attend_swz<SWZ, TOK>(r, 2 * i + (grp & 1)), a[0][0], a[0][1], a[0][2], a[0][3]);
+      ldsm_x4_trans(attend_swz_step<SWZ, TOK>(va, i), a[0][0], a[0][1], a[0][2], a[0][3]);
     }
   }
   // Zero the tokens at and past n: lo masks tokens 2t, 2t + 1, hi the tokens 8
@@ -378,12 +390,13 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
     ch[0][e] = G::kRawK ? c.bias[e & 1] : 0.f;
     ch[1][e] = 0.f;
   }
-  const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
+  const uint32_t ka = ks + attend_swz<G::kSwz, G::kTok>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
+  const uint32_t va = vs + VF::first(lane);
   if (G::kEight) {
 #pragma unroll
     for (int i = 0; i < KK / 2; ++i) {
       uint32_t x[4];
-      ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, 2 * i + (lane >> 4)), x[0], x[1], x[2], x[3]);
+      ldsm_x4(attend_swz_step<G::kSwz, G::kTok>(ka, i), x[0], x[1], x[2], x[3]);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         uint32_t a0, a1, a2, a3;
@@ -403,7 +416,7 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       uint32_t a0, a1, a2, a3;
-      ldsm_x4(ks + attend_swz<G::kSwz, G::kTok>(r, kk * 2 + (lane >> 4)), a0, a1, a2, a3);
+      ldsm_x4(attend_swz_step<G::kSwz, G::kTok>(ka, kk), a0, a1, a2, a3);
 #pragma unroll
       for (int q = 0; q < QT; ++q)
         MmaOp<T>::run(ch[kk & 1], a0, a1, a2, a3, c.q[kk][0][q], c.q[kk][1][q]);
@@ -478,7 +491,7 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
 #pragma unroll
     for (int i = 0; i < KK / VF::kPer; ++i) {
       VF v;
-      v.load(vs, i, lane);
+      v.load(va, i);
 #pragma unroll
       for (int q = 0; q < PT; ++q)
 #pragma unroll
@@ -505,7 +518,7 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
 #pragma unroll
     for (int i = 0; i < KK / VF::kPer; ++i) {
       VF v;
-      v.load(vs, i, lane);
+      v.load(va, i);
       v.mask(top - tok0, lane);
 #pragma unroll
       for (int k = 0; k < VF::kPer; ++k) {

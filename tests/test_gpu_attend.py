@@ -277,6 +277,52 @@ def test_diff_of_equal_maps_and_zero_lambda():
     c.check(c.run(), "lambda 0")
 
 
+# ---------------------------------------------------------------- shapes of the batch
+KINDS = [(I8, BF16, 1, 128), (F8, F32, 1, 64), (F16, F16, 2, 128), (F32, F32, 2, 48)]
+
+
+@pytest.mark.parametrize("kv,q_dt,maps,D", KINDS)
+def test_batches_of_many_sizes(kv, q_dt, maps, D):
+    """No context at all; more sequences than threads of a CTA; one long request; a
+    batch whose requests are mostly short beside a long one."""
+    g = torch.Generator().manual_seed(D)
+    many = torch.randint(0, 60, (900,), generator=g).tolist()
+    for lens in ([0, 0, 0], many + [700], [70001], [3] * 40 + [20000], [256] * 5, [257] * 5):
+        c = Case(lens, hq=2, hkv=1, D=D, kv=kv, q_dt=q_dt, maps=maps, seed=len(lens))
+        c.check(c.run(), f"{len(lens)} requests, longest {max(lens)}")
+
+
+@pytest.mark.parametrize("kv,q_dt,maps,D", KINDS)
+def test_a_prompt_of_new_rows(kv, q_dt, maps, D):
+    """Hundreds of causal rows of one request: many column chunks of one context."""
+    c = Case([330, 40], [300, 1], hq=4, hkv=2, D=D, kv=kv, q_dt=q_dt, maps=maps, seed=8)
+    want = c.append_reference()
+    out = c.run(step=True)
+    assert torch.equal(c.kc.view(torch.uint8), want[0].view(torch.uint8))
+    c.check(out, "300 rows")
+
+
+def test_the_bound_of_contexts_may_be_loose():
+    for maps, kv in ((1, I8), (2, F16)):
+        c = Case([100, 1, 3000], hq=8, hkv=2, kv=kv, q_dt=F16, maps=maps, seed=12)
+        c.max_ctx = 131072
+        c.check(c.run(), "loose")
+
+
+def test_zero_and_negative_score_scales():
+    for scale in (0.0, -0.2):
+        for maps, kv in ((1, F8), (2, BF16), (2, F32)):
+            c = Case([100, 17], hq=4, hkv=2, kv=kv, q_dt=F32, maps=maps, seed=13, norm=False)
+            c.scale = scale
+            out = c.run()
+            c.scale = scale
+            ref, tol = c.reference()
+            # (the bound's S is of |scale|)
+            c.scale = abs(scale)
+            tol = torch.maximum(tol, c.reference()[1])
+            assert bool(((out.double() - ref).abs() <= tol).all()), (scale, maps, kv)
+
+
 # ---------------------------------------------------------------- masked places
 @pytest.mark.parametrize("kv,maps", [(BF16, 2), (F16, 2), (F32, 2), (I8, 1), (F8, 1), (F8, 2)])
 @pytest.mark.parametrize("D", [128, 48])
