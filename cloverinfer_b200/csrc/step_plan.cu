@@ -14,8 +14,8 @@
 //
 // Bound: launch latency and three dependent loads (rows, lengths, block ids)
 // for a decode step; for admissions of whole prompts the 12 bytes written per
-// token (12 bytes of 228k tokens: 35 us from 8 CTAs of 512 threads, a round of
-// dependent loads per 16k tokens; 16 CTAs of 1024 threads: 11).  One thread-block
+// token (228k tokens, 48 requests: 35 us from 8 CTAs of 512 threads, a round of
+// dependent loads per 16k tokens; 16 from 16 CTAs of 1024 threads).  One thread-block
 // cluster: every CTA scans all items by itself (into
 // shared memory) and takes its share of the tokens, and the state that the
 // scans read (lengths, table lengths, stack top) is committed after the
