@@ -429,7 +429,10 @@ def kv_append_scaled(k_cache, v_cache, k_scales, v_scales, k_new, v_new, slot_ma
         raise ValueError(f"{what}: slot_mapping must be {n} contiguous int64 values")
     if n == 0:
         return
-    if (k_new.stride(-1) != 1 and d > 1) or (k_new.stride(-2) != d and h > 1) or v_new.stride() != k_new.stride():
+    k0, v0 = (x.select(-3, 0) for x in (k_new, v_new))
+    k0, v0 = (x[0] if many else x for x in (k0, v0))
+    if (not (k0.is_contiguous() and v0.is_contiguous()) or (n > 1 and v_new.stride(-3) != k_new.stride(-3))
+            or (many and v_new.stride(0) != k_new.stride(0))):
         raise ValueError(f"{what}: each token's [H, D] row must be contiguous")
     rc = _call_on(dev, lib().clover_b200_kv_append_scaled, k_cache.data_ptr(), v_cache.data_ptr(),
                   k_scales.data_ptr(), v_scales.data_ptr(), _DTYPE[k_cache.dtype],
@@ -468,7 +471,7 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
     rows, hq, dq = q.shape
     if dq != d or out.shape != q.shape:
         raise ValueError(f"{what}: q/out shape mismatch")
-    if q.stride(2) != 1 or q.stride(1) != d or out.stride(2) != 1 or out.stride(1) != d:
+    if rows and not (q[0].is_contiguous() and out[0].is_contiguous()):
         raise ValueError(f"{what}: each row's [Hq, D] must be contiguous")
     if out.dtype != q.dtype or v_cache.dtype != k_cache.dtype:
         raise TypeError(f"{what}: out dtype must equal q dtype, V's cache K's")
@@ -491,7 +494,8 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
             raise ValueError(f"{what}: new K/V must be [{rows}, {hkv}, {d}]")
         if v_new.dtype != k_new.dtype or (k_scales is None and k_new.dtype != k_cache.dtype):
             raise TypeError(f"{what}: new K/V dtype must match the cache")
-        if rows and (k_new.stride(2) != 1 or k_new.stride(1) != d or v_new.stride() != k_new.stride()):
+        if rows and not (k_new[0].is_contiguous() and v_new[0].is_contiguous()
+                         and (rows == 1 or v_new.stride(0) == k_new.stride(0))):
             raise ValueError(f"{what}: each token's [Hkv, D] row must be contiguous")
     if diff:
         if lam.dtype != torch.float32 or lam.shape != (hq,) or not lam.is_contiguous():
@@ -513,10 +517,12 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
             _attend_ws[key] = need
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    args = (out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), dtype_code(q.dtype),
-            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+    one = rows == 1  # (a single row's stride says nothing)
+    args = (out.data_ptr(), hq * d if one else out.stride(0), q.data_ptr(), hq * d if one else q.stride(0),
+            dtype_code(q.dtype), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales),
             dtype_code(k_cache.dtype), nb, bs, _ptr(k_new), _ptr(v_new),
-            0 if k_new is None else k_new.stride(0), 0 if k_new is None else dtype_code(k_new.dtype),
+            0 if k_new is None else hkv * d if one else k_new.stride(0),
+            0 if k_new is None else dtype_code(k_new.dtype),
             block_tables.data_ptr(), block_tables.stride(0), _ptr(seq_rows), query_start_loc.data_ptr(),
             ctx_lens.data_ptr(), n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d,
             float(score_scale))

@@ -230,6 +230,10 @@ plan_step_kernel(const PlanArgs a) {
       if (tid == 0) *a.free_top = top - s_pop[a.n];
     }
   }
+  // A decode launched right behind reads its layout before it waits for this
+  // kernel's completion (it may start when the last CTA ends): every write is
+  // performed by then.
+  __threadfence();
 }
 
 }  // namespace clover

@@ -225,7 +225,8 @@ class PagedKVPool:
 
     # ------------------------------------------------------------ plan on the GPU
     def set_seq_lens(self, rows: torch.Tensor, lens: torch.Tensor) -> None:
-        """Tell ``plan_step`` how many tokens rows hold (device int32 tensors)."""
+        """Tell ``plan_step`` how many tokens rows hold (device int32 tensors): once per
+        sequence, and again when its row goes to another one."""
         self.seq_lens.index_copy_(0, rows.long(), lens)
 
     def plan_step(self, rows: torch.Tensor, n_new: torch.Tensor, max_tokens: int) -> StepPlan:

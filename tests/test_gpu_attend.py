@@ -240,6 +240,17 @@ def test_scaled_strides_and_new_types():
         assert bool((o[:, 0] == 0).all())
 
 
+def test_single_rows_and_heads_of_any_stride():
+    """One row, one head: the strides of axes of length one say nothing."""
+    for maps, kv in ((1, I8), (2, F16)):
+        c = Case([90], hq=1, hkv=1, kv=kv, q_dt=F16, maps=maps, seed=6)
+        c.q, c.kn, c.vn = (x.as_strided(x.shape, (0, 7, 1)) for x in (c.q, c.kn, c.vn))
+        want = c.append_reference()
+        out = c.run(step=True)
+        assert torch.equal(c.kc.view(torch.uint8), want[0].view(torch.uint8))
+        c.check(out, "one row")
+
+
 # ---------------------------------------------------------------- differential decode
 @pytest.mark.parametrize("lens", [LENS, SHORT], ids=["long", "short"])
 @pytest.mark.parametrize("kv,q_dt", [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32), (F32, F32), (I8, BF16), (F8, F32)])
