@@ -28,8 +28,9 @@ struct AppendScaledArgs {
 // in flight; blockIdx.y is the layer, blockIdx.z K or V.  Bound: HBM (read the
 // row, write one byte per value), with the instructions close behind: one vector
 // per lane repeats the row's scale, slot and division in every lane (16381
-// tokens x 8 heads x 128, f16 -> e4m3: 46 us; a warp per row without vectors 92).
-constexpr int kAppendFlight = 2;
+// tokens x 8 heads x 128, f16 -> e4m3: 46 us; a warp per row without vectors 92;
+// this 21.5, 72 % of the copy peak).
+constexpr int kAppendFlight = 1;  // (2: 27.5 us, fewer warps on an SM)
 
 template <bool FP8, typename TI, int NV>
 __global__ void __launch_bounds__(256)
@@ -207,7 +208,6 @@ extern "C" int clover_b200_kv_append_scaled(
     int lpr = 1;
     while (lpr * 4 < vecs) lpr *= 2;
     const int64_t warps = (n_tokens * num_kv_heads + 32 / lpr - 1) / (32 / lpr);
-    // few rows: one in flight per thread, spread over the SMs
     const int64_t want_v = (warps + 7) / 8;
     const int64_t cap_v = (148 * 16 + 2 * n_layers - 1) / (2 * n_layers);
     const dim3 gv((unsigned)(want_v < cap_v ? want_v : cap_v), (unsigned)n_layers, 2);
