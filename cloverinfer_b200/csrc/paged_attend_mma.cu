@@ -623,7 +623,7 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
 // Fused append: the new tokens of a sequence (rows row0 .. row0 + nq - 1) that
 // lie in the unit [tok0, tok0 + 16 SUBS), for KV head kvh, written by the warp
 // before the unit is copied (slot0, slot1: first cache slot of its 16-token
-// steps).
+// steps, negative where the step's block id is bad: its tokens are skipped).
 template <int KV, int D, int SUBS>
 __device__ __forceinline__ void append_unit(const AttendArgs& a, int row0, int nq, int ctx, int tok0, int kvh,
                                             int slot0, int slot1, int lane) {
@@ -631,7 +631,9 @@ __device__ __forceinline__ void append_unit(const AttendArgs& a, int row0, int n
     const int r = row0 + j;
     const int rel = __ldg(a.ctx + r) - 1 - tok0;
     if (rel < 0 || rel >= SUBS * kUnitTok || rel + tok0 >= ctx) continue;
-    const int64_t at = (rel < kUnitTok ? slot0 : slot1) + (rel & (kUnitTok - 1));
+    const int first = rel < kUnitTok ? slot0 : slot1;
+    if (first < 0) continue;
+    const int64_t at = first + (rel & (kUnitTok - 1));
     const int64_t row = (at * a.hkv + kvh) * D, src = (int64_t)r * a.new_stride + (int64_t)kvh * D;
     if (KV >= KV_I8) {
       uint8_t* kd = static_cast<uint8_t*>(const_cast<void*>(a.kc)) + row;
@@ -657,7 +659,8 @@ __device__ __forceinline__ void append_unit(const AttendArgs& a, int row0, int n
 }
 
 // The copies of a ring: the unit after the last one issued, and where its
-// tokens are.  Block ids are held 32 at a time (lane i: block id_base + i).
+// tokens are.  Block ids are held 32 at a time (lane i: block id_base + i), a
+// bad one as -1.
 template <int KV, bool QF32, int D, int CW>
 struct RingCopies {
   using G = AttendGeom<KV, QF32, D, CW>;
@@ -689,24 +692,29 @@ struct RingCopies {
         ids = blk + lane < a.table_stride ? __ldg(a.tables + (int64_t)trow * a.table_stride + blk + lane) : -1;
         if (ids < 0 || ids >= a.num_blocks) {
           raise_status(a.status, CLOVER_B200_DEV_BAD_BLOCK);
-          ids = 0;  // keep the pipeline well-formed; the output is flagged
+          ids = -1;
         }
       }
     }
-    int slot[SUBS];  // first cache slot of each 16-token step
+    // First cache slot of each 16-token step: what is copied (a bad block reads
+    // block 0, so that the pipeline stays well-formed; the output is flagged),
+    // and what an append may write to (a bad block: nothing).
+    int slot[SUBS], own[SUBS];
     int id[SUBS], off[SUBS];
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
-      id[u] = __shfl_sync(0xffffffffu, ids, blk - id_base);
+      const int got = __shfl_sync(0xffffffffu, ids, blk - id_base);
+      id[u] = max(got, 0);
       off[u] = sub * kUnitTok;
       slot[u] = id[u] * a.bs + off[u];
+      own[u] = got < 0 ? -1 : slot[u];
       if (++sub == upb) {
         sub = 0;
         ++blk;
       }
     }
     if (a.k_new != nullptr && (cur.jj + 1) * G::kTok > first_new)
-      append_unit<KV, D, SUBS>(a, cur.s.row0, cur.s.nq, cur.s.ctx, cur.jj * G::kTok, kvh, slot[0], slot[SUBS - 1],
+      append_unit<KV, D, SUBS>(a, cur.s.row0, cur.s.nq, cur.s.ctx, cur.jj * G::kTok, kvh, own[0], own[SUBS - 1],
                                lane);
     const int left = (cur.s.ctx + kUnitTok - 1) / kUnitTok - cur.jj * SUBS;  // steps of the segment
     const int subs = left < SUBS ? left : SUBS;
