@@ -77,6 +77,7 @@ class _Stats:
 @dataclass
 class PlannedStep:
     """A step planned by ``begin_step``: one for all layers."""
+    request_ids: List[str]
     reqs: List[_Request]
     n_new: List[int]
     targets: List[int]
@@ -709,13 +710,15 @@ class B200AttentionBackend:
             if n:
                 pool.row_blocks[r] = max(pool.row_blocks[r], pool.blocks_for(t))
         pool.free_count -= need
-        return PlannedStep(reqs, n_new, targets, p.rows, p.query_start_loc, p.ctx_lens, p.slots)
+        return PlannedStep(list(request_ids), reqs, n_new, targets, p.rows, p.query_start_loc, p.ctx_lens, p.slots)
 
     def decode_planned(self, step: PlannedStep, layer_idx: int, query: torch.Tensor, key: torch.Tensor,
                        value: torch.Tensor, score_scale: float = 1.0,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One layer of a planned step: append its new K/V and attend.  Tensors, result and
-        ``out`` as in ``decode_batch``."""
+        ``out`` as in ``decode_batch``.  KeyError, before anything changes, if a request of the
+        step has been freed since (its table row may be another request's by now); the others'
+        remaining layers then go through ``decode_batch``."""
         if not 0 <= layer_idx < self.num_layers:
             raise IndexError(f"layer_idx {layer_idx} out of range [0, {self.num_layers})")
         T = sum(step.n_new)
@@ -724,6 +727,9 @@ class B200AttentionBackend:
             raise ValueError(f"expected {T} new tokens, got q {tuple(query.shape)} k {tuple(key.shape)}")
         if hq % self.num_kv_heads or d != self.head_dim:
             raise ValueError(f"query heads x dim {hq} x {d} do not fit {self.num_kv_heads} KV heads x {self.head_dim}")
+        for rid, r in zip(step.request_ids, step.reqs):
+            if self._reqs.get(rid) is not r:
+                raise KeyError(f"request {rid} was freed inside the step")
         for r, t, n in zip(step.reqs, step.targets, step.n_new):
             if r.layer_len[layer_idx] != t - n:
                 raise RuntimeError(f"layer {layer_idx} of the step has run already, or its requests went on")

@@ -1,0 +1,51 @@
+"""Host rules of the backend's planned steps and of differential layers, on a
+backend object without a GPU: nothing below launches anything."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cloverinfer_b200 import B200AttentionBackend
+from cloverinfer_b200.backend import PlannedStep, _Request
+
+
+def bare(layers=2, hkv=2, D=64):
+    """A backend's host state: requests "a" and "b" with 5 and 9 tokens, and a
+    launch that only says that it was reached."""
+    be = B200AttentionBackend.__new__(B200AttentionBackend)
+    be.num_layers, be.num_kv_heads, be.head_dim, be.device = layers, hkv, D, torch.device("cpu")
+    be._pending_ingest, be._peer = [], None
+    be._reqs = {"a": _Request(0, [5] * layers, 5), "b": _Request(1, [9] * layers, 9)}
+
+    def launch(reqs, layer, n_new, targets, query, *rest, **kw):
+        for r, n in zip(reqs, n_new):
+            r.layer_len[layer] += n
+        return query
+
+    be._launch = launch
+    return be
+
+
+def planned(be):
+    ids = list(be._reqs)
+    reqs = [be._reqs[r] for r in ids]
+    n = [1] * len(ids)
+    e = torch.zeros(0, dtype=torch.int32)
+    return PlannedStep(request_ids=ids, reqs=reqs, n_new=n, targets=[r.layer_len[0] + 1 for r in reqs], rows=e,
+                       query_start_loc=e, ctx_lens=e, slots=e)
+
+
+def test_a_planned_step_refuses_requests_that_left():
+    x, kv = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64)
+    for again in (False, True):
+        be = bare()
+        step = planned(be)
+        assert be.decode_planned(step, 0, x, kv, kv).shape == x.shape
+        gone = be._reqs.pop("a")  # freed between two layers of the step
+        if again:  # and its id taken by another request of the same length
+            be._reqs["a"] = _Request(gone.row, list(gone.layer_len), gone.ctx)
+        held = {r: list(q.layer_len) for r, q in be._reqs.items()}
+        with pytest.raises(KeyError):
+            be.decode_planned(step, 1, x, kv, kv)
+        assert {r: q.layer_len for r, q in be._reqs.items()} == held
