@@ -27,6 +27,11 @@
 //     in one word; the conversion picks the bytes of one dim, so M row g is dim
 //     2g and row g + 8 dim 2g + 1.
 //   * int8: byte ^ 0x80 under 0x64 is the fp16 1024 + 128 + x; subtract 1152.
+//     (K's codes left 1152 high, with that times the query's sum taken off each
+//     score, save two subtractions per four codes: 121.2 against 123.6 us on 64
+//     ragged requests of 1-4 rows.  But the partial sums are then about
+//     1152 |sum q| and round accordingly: 128 dims of mean and deviation 8 put
+//     scores off by up to 5e-4, against 6e-6 as here.)
 //     e4m3: the conversion instruction.
 // K's scale multiplies the score; V's scale multiplies the softmax weight.  The
 // weights' reference is a bound of score + e, 2^e >= V's scale: a weight times
@@ -71,10 +76,6 @@ struct AttendGeom {
   static constexpr int kScales = kEight ? 2 * kTok * 4 : 0;
   static constexpr int kStageB = kTiles + kScales;
   static constexpr int kQTerms = !QF32 ? 1 : KV == KV_BF16 ? 3 : 2;
-  // int8 K codes enter the product 1152 high, and the score's chain starts at
-  // -1152 times the sum of the query: two subtractions less per four codes.  It
-  // costs about 2^-24 * 1152 |sum q| of the score, so not under fp32 queries.
-  static constexpr bool kRawK = KV == KV_I8 && !QF32;
   static constexpr int kPTerms = KV == KV_BF16 && QF32 ? 3 : 2;
   // Warps: 16, 12 or 8 (128, 168 or 255 registers each), as many as hold
   // accumulators, query fragments and about 80 more, with rings at least two
@@ -120,18 +121,15 @@ __device__ __forceinline__ uint32_t hsub2_u(uint32_t a, uint32_t b) {
   asm("sub.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// Two fp16 pairs from four codes, in the order bytes (0, 2), (1, 3).  RAW: int8
-// codes stay 1152 higher (the caller's sum takes that off).
-template <int KV, bool RAW = false>
+// Two fp16 pairs from four codes, in the order bytes (0, 2), (1, 3).
+template <int KV>
 __device__ __forceinline__ void codes_to_f16(uint32_t x, uint32_t& lo, uint32_t& hi) {
   if (KV == KV_I8) {
     const uint32_t u = x ^ 0x80808080u;
     lo = prmt(u, 0x64646464u, 0x4240u);
     hi = prmt(u, 0x64646464u, 0x4341u);
-    if (!RAW) {
-      lo = hsub2_u(lo, 0x64806480u);
-      hi = hsub2_u(hi, 0x64806480u);
-    }
+    lo = hsub2_u(lo, 0x64806480u);
+    hi = hsub2_u(hi, 0x64806480u);
   } else {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
         "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
@@ -190,7 +188,6 @@ struct AttendCols {
   uint32_t q[D / 16][2][G::kQTerms];
   float acc[D / 16][4];
   float m[2], l[2], sc[2];  // sc: score scale in base 2
-  float bias[2];  // int8, 16-bit queries: -1152 * sum of the column's query
   int lim[2];
   int min_lim;  // least limit of the warp's columns
 };
@@ -276,18 +273,6 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
     split_terms<T, G::kQTerms>(x[kk][0], x[kk][1], c.q[kk][0]);
     split_terms<T, G::kQTerms>(x[kk][2], x[kk][3], c.q[kk][1]);
   }
-  float total = 0.f;
-  if (G::kRawK) {  // of the values as the fragments hold them
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 f = Pack<T>::unpack(c.q[kk][i][0]);
-        total += f.x + f.y;
-      }
-    total += __shfl_xor_sync(0xffffffffu, total, 1);
-    total += __shfl_xor_sync(0xffffffffu, total, 2);
-  }
   // limits and score scales of columns 2t, 2t + 1 from the lanes that hold them
   int lim = ci.valid ? ci.lim : 0;
   if (lim > cap) {  // a row past its sequence's last row
@@ -300,7 +285,6 @@ __device__ __forceinline__ void load_columns(const AttendArgs& a, const Cursor& 
     const int src = ((lane & 3) * 2 + e) * 4;
     c.lim[e] = __shfl_sync(0xffffffffu, lim, src);
     c.sc[e] = a.scale_log2 * __shfl_sync(0xffffffffu, inv, src);
-    c.bias[e] = -1152.f * __shfl_sync(0xffffffffu, total, src);
     c.m[e] = kNoRef;
     c.l[e] = 0.f;
   }
@@ -386,10 +370,7 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
   // ---- S = K . Q^T (two chains), times K's scale
   float ch[2][4], s[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    ch[0][e] = G::kRawK ? c.bias[e & 1] : 0.f;
-    ch[1][e] = 0.f;
-  }
+  for (int e = 0; e < 4; ++e) ch[0][e] = ch[1][e] = 0.f;
   const uint32_t ka = ks + attend_swz<G::kSwz, G::kTok>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
   const uint32_t va = vs + VF::first(lane);
   if (G::kEight) {
@@ -404,8 +385,8 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
           e4m3_to_f16(x[2 * k], a0, a2);
           e4m3_to_f16(x[2 * k + 1], a1, a3);
         } else {
-          codes_to_f16<KV, G::kRawK>(x[2 * k], a0, a2);
-          codes_to_f16<KV, G::kRawK>(x[2 * k + 1], a1, a3);
+          codes_to_f16<KV>(x[2 * k], a0, a2);
+          codes_to_f16<KV>(x[2 * k + 1], a1, a3);
         }
 #pragma unroll
         for (int q = 0; q < QT; ++q)

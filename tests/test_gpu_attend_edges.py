@@ -47,3 +47,26 @@ def test_an_append_to_a_bad_page_writes_nothing(kv, maps, D, bad):
         if ks is not None:
             assert torch.equal(c.ks, ks) and torch.equal(c.vs, vs), (lens, new)
         assert bool(torch.isfinite(out[new[0]:c.T]).all())
+
+
+# ---------------------------------------------------------------- queries far from zero mean
+@pytest.mark.parametrize("q_dt", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_int8_scores_of_queries_with_a_mean(D, maps, q_dt):
+    """Queries around 8, keys with one dim each: the products that a score sums are
+    one large value and zeros, whose sum rounds (and so may the bound) by next to
+    nothing, while the sum of the query over all dims is D times as large."""
+    c = Case([5] * 24 + [200], hq=16, hkv=4, D=D, kv=I8, q_dt=q_dt, maps=maps, seed=41, norm=False)
+    g = torch.Generator().manual_seed(42)
+    c.q = (8 + 0.02 * torch.randn(c.q.shape, generator=g)).to(q_dt).cuda()
+    # token t of a block: code 127 at a dim of its own (in each half for two maps)
+    codes = torch.zeros(c.nb, c.bs, c.hkv, D, dtype=I8)
+    at = torch.randint(0, D // maps, (c.nb, c.bs, c.hkv), generator=g)
+    for m in range(maps):
+        codes.scatter_(3, (at + m * (D // 2))[..., None], 127)
+    c.kc = codes.cuda()
+    c.ks.fill_(1 / 127)
+    c.vs.fill_(1 / 127)
+    c.scale = 120.0  # scores near 960, which rounding may move by (D + 8) 2^-24 of that
+    c.check(c.run(), f"D{D} {q_dt}")
