@@ -35,17 +35,24 @@
 //     e4m3: the conversion instruction.
 // K's scale multiplies the score; V's scale multiplies the softmax weight.  The
 // weights' reference is a bound of score + e, 2^e >= V's scale: a weight times
-// its scale is then bounded, so fp16 holds it whatever the scales are, and only
-// one exponential is needed.  Weights are split into hi + lo 16-bit terms (2^-16
-// of the weight in bf16, 2^-22 in fp16; three terms, 2^-24, for fp32 queries
-// over bf16).  fp32 queries are split the same way; columns of fp16 products are
-// first scaled by a power of two so that their largest value is in
-// [2^14, 2^15).
+// its scale is then bounded, so fp16 does not overflow whatever the scales are,
+// and only one exponential is needed.  Weights are split into two 16-bit terms:
+// 2^-16 of the weight in bf16 (three terms, 2^-24, for fp32 queries); 2^-22 in
+// fp16 down to 2^-3, and half of fp16's least step, 2^-25, below.  fp16 weights
+// therefore stand high: a move of the reference puts the largest at 2^12, so
+// what is lost of a small one is at most 2^-37 of it.  (At 2^0, 40000 tokens
+// 18 nats below one with a V row of its own lost all that shared its piece, 9 to
+// 23 % of their sum; the sum of the weights itself is in fp32.)  fp32 queries are
+// split the same way (2^-22 of the column's largest over fp16 products, 2^-24
+// over bf16); columns of fp16 products are first scaled by a power of two so that
+// their largest value is in [2^14, 2^15).
 //
-// The reference moves only when a weight exceeds it by more than 2^8 (far inside
-// fp16 and fp32): with the running maximum itself about half of the stages of a
-// worker rescaled the accumulators, and every stage took the columns' maxima
-// over the lanes.
+// The reference moves only when a weight outgrows it: 2^15 for fp16 (2^3 above
+// the last move), 2^8 for bf16.  With the running maximum itself about half of
+// the stages of a worker rescaled the accumulators, and every stage took the
+// columns' maxima over the lanes; 2^8, 2^5 and 2^3 of room measure alike (64
+// ragged requests 124.0, 124.1, 124.1 us; scores five times as wide 124.4,
+// 124.6, 125.1).
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -77,6 +84,10 @@ struct AttendGeom {
   static constexpr int kStageB = kTiles + kScales;
   static constexpr int kQTerms = !QF32 ? 1 : KV == KV_BF16 ? 3 : 2;
   static constexpr int kPTerms = KV == KV_BF16 && QF32 ? 3 : 2;
+  // Where a move of the reference puts the largest weight (log2), and the weight
+  // that makes it move.
+  static constexpr float kTopLog2 = KV == KV_BF16 ? 0.f : 12.f;
+  static constexpr float kMaxWeight = KV == KV_BF16 ? 256.f : 32768.f;
   // Warps: 16, 12 or 8 (128, 168 or 255 registers each), as many as hold
   // accumulators, query fragments and about 80 more, with rings at least two
   // stages deep.
@@ -144,12 +155,6 @@ __device__ __forceinline__ void e4m3_to_f16(uint32_t x, uint32_t& lo, uint32_t& 
       : "=r"(lo), "=r"(hi)
       : "r"(x));
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -173,6 +178,11 @@ __device__ __forceinline__ void split_terms(float x0, float x1, uint32_t (&out)[
 // A reference below every score (finite, so that differences to -inf stay
 // -inf): the weights of a column that has seen nothing are 2^-inf.
 constexpr float kNoRef = -1e30f;
+
+// V scales under 2^-80 count as that in the reference (a zero row's is 0, the
+// least stored 2^-109), though the weight takes them as they are: a softmax
+// weight is then at most 2^(15 + 80), and the sum of 2^31 of them finite.
+constexpr float kLeastScale = 8.271806125530277e-25f;
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -403,11 +413,14 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
         MmaOp<T>::run(ch[kk & 1], a0, a1, a2, a3, c.q[kk][0][q], c.q[kk][1][q]);
     }
   }
-  float vsc[2] = {1.f, 1.f};
+  // V's scales, and their bounds for the reference
+  float vsc[2] = {1.f, 1.f}, vref[2] = {1.f, 1.f};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    // V scales under 2^-110 (zero rows; 2^-107 is the least stored) count as that
-    if (G::kEight) vsc[h] = max_nan(scales[G::kTok + g + 8 * h], 7.703719777548943e-34f);
+    if (G::kEight) {
+      vsc[h] = scales[G::kTok + g + 8 * h];
+      vref[h] = fmaxf(fabsf(vsc[h]), kLeastScale);
+    }
     const float ksc = G::kEight ? scales[g + 8 * h] : 1.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -433,18 +446,18 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       weigh(h, e);
-      big = fmaxf(big, w[2 * h + e]);
+      big = fmaxf(big, p[2 * h + e] * vref[h]);
     }
-  if (__any_sync(0xffffffffu, big > 256.f)) {
+  if (__any_sync(0xffffffffu, big > G::kMaxWeight)) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float mx = -INFINITY;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (!masked(h, e)) mx = fmaxf(mx, fmaf(s[2 * h + e], c.sc[e], G::kEight ? fast_log2(vsc[h]) : 0.f));
+        if (!masked(h, e)) mx = fmaxf(mx, fmaf(s[2 * h + e], c.sc[e], G::kEight ? fast_log2(vref[h]) : 0.f));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float nm = fmaxf(c.m[e], mx);
+      const float nm = fmaxf(c.m[e], mx - G::kTopLog2);
       const float al = fast_exp2(c.m[e] - nm);
       c.m[e] = nm;
       c.l[e] *= al;

@@ -4,11 +4,13 @@ arguments allow.  Attention is held to the bound of test_gpu_attend."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 from conftest import gpu
-from test_gpu_attend import BF16, F16, F32, F8, I8, Case
+from test_gpu_attend import BF16, F16, F32, F8, I8, Case, quantise
 
 pytestmark = gpu
 
@@ -70,3 +72,93 @@ def test_int8_scores_of_queries_with_a_mean(D, maps, q_dt):
     c.vs.fill_(1 / 127)
     c.scale = 120.0  # scores near 960, which rounding may move by (D + 8) 2^-24 of that
     c.check(c.run(), f"D{D} {q_dt}")
+
+
+# ---------------------------------------------------------------- weights of very different size
+def repeated(c, times):
+    """The one-request case as a batch of equal requests over the same blocks: enough
+    work that a worker's piece of a context is thousands of tokens long.  (c.reference
+    stays that of one.)"""
+    n = c.lens[0]
+    c.q = c.q[:1].repeat(times, 1, 1)
+    c.tables = c.tables[:1].repeat(times, 1)
+    c.qsl = torch.arange(times + 1, dtype=torch.int32, device="cuda")
+    c.ctx = torch.full((times,), n, dtype=torch.int32, device="cuda")
+    return c
+
+
+SPIKE_KINDS = [(F16, 2), (I8, 1), (F8, 1), (I8, 2), (BF16, 2)]
+
+
+@pytest.mark.parametrize("kv,maps", SPIKE_KINDS)
+@pytest.mark.parametrize("bits", [12.3, 19.6, 26.1])
+def test_many_small_weights_beside_a_large_one(kv, maps, bits):
+    """One token 2^bits above 40000 equal ones: its V row has dim 0 alone, theirs the
+    other dims, so those hold nothing but the small weights.  (192 such requests: the
+    token's piece holds about a tenth of them.)  Bound, relative: an fp16
+    weight is held to 2^-22, or by half of fp16's least step, 2^-25, where the largest
+    weight is at least 2^12; the score, the base-2 exponential and the sums as in
+    test_gpu_attend."""
+    n, D, at = 40000, 128, 777
+    c = Case([n], hq=8, hkv=1, D=D, kv=kv, q_dt=F32, maps=maps, seed=51, norm=False)
+    w = D // maps
+    half = torch.zeros(D, dtype=torch.float64)
+    half[::w] = 1.0  # one dim of each map carries the score
+    c.q = torch.zeros_like(c.q)
+    c.q[..., ::w] = 1.0
+    c.scale = 1.0
+    nats = bits * math.log(2.0)
+    k, v = torch.zeros(n, D), torch.ones(n, D)
+    v[:, 0] = 0
+    k[at] = half.float() * nats
+    v[at] = 0
+    v[at, 0] = 1.0
+    g = torch.Generator().manual_seed(52)
+    k[:, 3] = torch.rand(n, generator=g) - 0.5  # (rows without a score; q is 0 there)
+    blocks = c.tables[0, :-(-n // c.bs)].long()
+    pad = lambda x: torch.cat([x, torch.zeros(len(blocks) * c.bs - n, D)]).view(-1, c.bs, 1, D)  # noqa: E731
+    for cache, scales, x in ((c.kc, c.ks, pad(k)), (c.vc, c.vs, pad(v))):
+        if scales is None:
+            cache[blocks] = x.to(kv).cuda()
+        else:
+            code, s = quantise(x, kv)
+            cache.view(torch.uint8)[blocks] = code.view(torch.uint8).cuda()
+            scales[blocks] = s.transpose(1, 2).cuda()
+    c.lam.zero_()
+    out = repeated(c, 192).run().double()
+    torch.cuda.synchronize()
+    assert int(c.status.item()) == 0
+    ref, _ = c.reference()
+    delta = (D + 8) * 2.0 ** -24 * nats
+    small = 2.0 ** -bits * 2.0 ** 12
+    rel = 2 * delta + 2.0 ** -20 + (n + 64) * 2.0 ** -24 + max(2.0 ** -22, 2.0 ** -25 / small)
+    err = ((out - ref).abs() / ref.abs())[..., 1:].max()
+    assert float(err) <= rel, f"{kv} {bits}: {float(err):.3g} of the small weights' sum, bound {rel:.3g}"
+    assert float(((out - ref).abs() / ref.abs())[..., 0].max()) <= rel
+
+
+@pytest.mark.parametrize("kv", [I8, F8])
+@pytest.mark.parametrize("q_dt", [F32, BF16])
+def test_zero_and_tiny_value_rows(kv, q_dt):
+    """Thousands of zero V rows with the largest scores before the others; V rows so
+    small that a weight times their scale is far below fp16."""
+    c = Case([6000, 40, 3000], hq=8, hkv=2, kv=kv, q_dt=q_dt, seed=61, spread=False)
+    ids = c.tables[0, :300].long()  # 4800 tokens
+    c.vc.view(torch.uint8)[ids] = 0
+    c.vs[ids] = 0
+    c.check(c.run(), "zeros first")
+    one = Case([6000], hq=8, hkv=2, kv=kv, q_dt=q_dt, seed=61, spread=False)
+    one.vc.view(torch.uint8)[one.tables[0, :300].long()] = 0
+    one.vs[one.tables[0, :300].long()] = 0
+    one.check(repeated(one, 1200).run()[-1:], "zeros first, pieces of whole contexts")
+    c.vc.view(torch.uint8)[c.tables[2, :188].long()] = 0
+    c.vs[c.tables[2, :188].long()] = 0
+    out = c.run()
+    c.check(out, "nothing but zeros")
+    assert bool((out[2] == 0).all())
+    for e in (-40, -84):
+        c = Case([700, 40, 100], hq=8, hkv=2, kv=kv, q_dt=q_dt, seed=62, spread=False)
+        c.vs *= 2.0 ** e
+        c.check(c.run(), f"V of 2^{e}")
+        c.vs[c.tables[0, 7]] *= 2.0 ** 60  # a block of a far larger size among them
+        c.check(c.run(), f"V of 2^{e} beside larger")
