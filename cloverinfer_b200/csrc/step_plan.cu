@@ -20,6 +20,8 @@
 // shared memory) and takes its share of the tokens, and the state that the
 // scans read (lengths, table lengths, stack top) is committed after the
 // cluster barrier, so no global counter or scratch memory is needed.
+#include <mutex>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -236,6 +238,35 @@ plan_step_kernel(const PlanArgs a) {
   __threadfence();
 }
 
+// ------------------------------------------------------------------ host side
+// Shared memory of a plan: five words per item and two more, a bit per row.
+static size_t plan_smem(int64_t items, int64_t rows) {
+  return (size_t)(2 * (items + 1) + 3 * items + (rows + 31) / 32) * 4;
+}
+
+// Lets the kernel have what the largest plan takes.  These limits are the
+// process's, not a call's, so they are set once per device and never lowered
+// under another thread's launch.
+template <int kPlanThreads>
+static int plan_configure() {
+  static std::mutex mu;
+  static uint64_t done = 0;  // one bit per device ordinal
+  int dev = 0;
+  int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 64 && (done >> dev & 1)) return CLOVER_B200_OK;
+  rc = check_cuda(cudaFuncSetAttribute(plan_step_kernel<kPlanThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)plan_smem(kPlanMaxItems, kPlanMaxRows)),
+                  "plan_step shared memory");
+  if (!rc)
+    rc = check_cuda(cudaFuncSetAttribute(plan_step_kernel<kPlanThreads>,
+                                         cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                    "plan_step cluster size");
+  if (!rc && dev < 64) done |= 1ull << dev;
+  return rc;
+}
+
 }  // namespace clover
 
 using namespace clover;
@@ -272,21 +303,15 @@ extern "C" int clover_b200_plan_step(int32_t* free_stack, int32_t* free_top, int
              max_tokens,
              ((reinterpret_cast<uintptr_t>(ctx_lens) | reinterpret_cast<uintptr_t>(slot_mapping)) & 15) == 0,
              dev_status};
-  const size_t smem = (size_t)(2 * (n_items + 1) + 3 * n_items + (num_rows + 31) / 32) * 4;
+  const size_t smem = plan_smem(n_items, num_rows);
   // One small CTA covers a decode step; admissions take up to 16 large ones.
   const bool small = max_tokens <= 4 * kPlanSmall * kPlanGroup && n_items <= 4 * kPlanSmall;
   const int threads = small ? kPlanSmall : kPlanLarge;
   int ctas = 1;
   while (!small && ctas < 16 && (int64_t)ctas * threads * kPlanGroup < max_tokens) ctas *= 2;
   void (*kern)(PlanArgs) = small ? plan_step_kernel<kPlanSmall> : plan_step_kernel<kPlanLarge>;
-  if (smem > 40 * 1024) {
-    const int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                              "plan_step shared memory");
-    if (rc) return rc;
-  }
-  if (ctas > 8) {
-    const int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                              "plan_step cluster size");
+  if (smem > 40 * 1024 || ctas > 8) {  // beyond what every kernel may have
+    const int rc = small ? plan_configure<kPlanSmall>() : plan_configure<kPlanLarge>();
     if (rc) return rc;
   }
   cudaLaunchConfig_t cfg = {};

@@ -55,3 +55,38 @@ def test_a_step_without_requests_or_tokens():
         assert be.decode_planned(step, 0, e, kv, kv).shape == (0, 4, 64)
     assert be.get_context_len("a") == 40
     be.pool.check_status()
+
+
+def test_plans_of_different_sizes_from_two_threads():
+    """The kernel's shared-memory limit is the process's: a call of one size must not
+    lower it under another's launch."""
+    import threading
+
+    import cloverinfer_b200 as cb
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def state(items, rows):
+        return (torch.arange(64, **i32), torch.tensor([64], **i32), torch.full((rows, 2), -1, **i32),
+                torch.zeros(rows, **i32), torch.zeros(rows, **i32), torch.arange(items, **i32),
+                torch.zeros(items, **i32), 16, torch.zeros(items + 1, **i32), torch.zeros(1, **i32),
+                torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, **i32))
+
+    states, failed = [state(8192, 1 << 18), state(2048, 4096)], []
+    torch.cuda.synchronize()
+
+    def run(s):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(1500):
+                    cb.plan_step(*s)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(s,)) for s in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed[0]
+    assert all(int(s[-1].item()) == 0 for s in states)
