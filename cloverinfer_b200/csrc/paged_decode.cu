@@ -238,6 +238,7 @@ paged_decode_mma_kernel(const __grid_constant__ CUtensorMap tmK,
   w.chunk = blockIdx.y - w.kvh * a.col_chunks;
   w.row0 = a.rows_identity ? w.b : __ldg(a.qsl + w.b);
   w.nq = a.rows_identity ? 1 : __ldg(a.qsl + w.b + 1) - w.row0;
+  // (a negative table row is a plan's padding: a sequence without tokens)
   const int trow = a.seq_rows ? __ldg(a.seq_rows + w.b) : w.b;
   // after a bounded wait gave up anywhere, later CTAs stop at once
   const int stat = a.status != nullptr ? *(volatile int32_t*)a.status : 0;
@@ -246,8 +247,11 @@ paged_decode_mma_kernel(const __grid_constant__ CUtensorMap tmK,
   const int c0 = w.chunk * CCOLS;
   // (Every CTA waits before it ends, early exits too: a grid that finished
   // before its predecessor would let the next kernel's wait pass early.)
-  if ((stat & CLOVER_B200_DEV_TIMEOUT) || w.nq <= 0 || c0 >= w.nq * a.group) {
+  if ((stat & CLOVER_B200_DEV_TIMEOUT) || w.nq <= 0 || c0 >= w.nq * a.group || trow < 0) {
     pdl_wait();
+    // padding taken for a row's sequence, before sequences that have rows
+    if (trow < 0 && w.nq > 0 && threadIdx.x == 0 && __ldg(a.qsl + w.b) < __ldg(a.qsl + a.n_seqs))
+      raise_status(a.status, CLOVER_B200_DEV_BAD_PLAN);
     pdl_trigger();
     return;
   }

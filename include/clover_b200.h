@@ -60,7 +60,9 @@ extern "C" {
 #define CLOVER_B200_DEV_TIMEOUT      0x10  /* a bounded wait gave up                */
 #define CLOVER_B200_DEV_CTX_RANGE    0x20  /* a context exceeds max_ctx_len        */
 #define CLOVER_B200_DEV_BAD_PLAN     0x40  /* plan_step: a row out of range or twice, a
-                                              negative count, too many tokens (nothing changed) */
+                                              negative count, too many tokens (nothing changed);
+                                              a decode told max_queries_per_seq = 1 over a batch
+                                              with padding before other sequences */
 
 /* ---- dtypes --------------------------------------------------------------- */
 #define CLOVER_B200_F32  0
@@ -225,7 +227,13 @@ CLOVER_B200_API int clover_b200_decode_partition_tokens(int32_t n_seqs, int32_t 
  * query_start_loc[b] .. query_start_loc[b+1]-1 (one row per new token; a
  * plain decode step has query_start_loc = 0,1,..,n_seqs) and block-table row
  * seq_rows ? seq_rows[b] : b.  Query row r attends causally to tokens
- * [0, ctx_lens[r]) of its sequence.
+ * [0, ctx_lens[r]) of its sequence.  With max_queries_per_seq = 1 and n_seqs
+ * rows, row b is taken for sequence b: where sequences without rows may stand
+ * before others (padding or counts of zero inside a clover_b200_plan_step),
+ * pass 2 or more.  A negative seq_rows[b] is padding: nothing is read or
+ * written for it, and before other sequences, where row b would be another's,
+ * it raises BAD_PLAN.  (A sequence with a table row and no query row is not
+ * noticed.)
  *
  *   q   [n_rows, num_q_heads, head_dim]  row stride q_row_stride elements,
  *                                          dtype q_dtype (F32 or kv_dtype)

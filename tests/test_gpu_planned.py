@@ -90,3 +90,61 @@ def test_plans_of_different_sizes_from_two_threads():
     torch.cuda.synchronize()
     assert not failed, failed[0]
     assert all(int(s[-1].item()) == 0 for s in states)
+
+
+@pytest.mark.parametrize("D", [64, 48])  # the tensor-core kernel, the other one
+def test_padding_and_one_row_per_sequence(D):
+    """max_q = 1 with as many rows as sequences takes row b for sequence b: padding
+    behind the last row is fine, padding before one is flagged (D = 48 reads the rows'
+    offsets and answers it), and max_q = 2 answers either.  Padding's own output rows
+    stay as they were."""
+    from cloverinfer_b200 import PagedKVPool, _lib
+    hq, hkv = 4, 2
+    pool = PagedKVPool(32, 16, hkv, D, max_seqs=4, dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(1)
+    rnd = lambda n, h: torch.randn(n, h, D, generator=g).bfloat16().cuda()  # noqa: E731
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    p = pool.plan_step(i32([0, 1, 2]), i32([30, 9, 50]), 89)
+    pool.append(0, rnd(89, hkv), rnd(89, hkv), p.slots)
+    q = rnd(3, hq)
+    for rows, good in (([2, 0, -1], True), ([-1, 2, 0], False), ([2, -1, 0], False), ([-1, 2], False), ([1, -1], True),
+                       ([-1, -1], True)):
+        n = len(rows)
+        p = pool.plan_step(i32(rows), i32([1] * n), n)
+        new = rnd(n, hkv)
+        pool.append(0, new, new, p.slots)
+        want = pool.decode(0, q[:n], p.query_start_loc, p.ctx_lens, p.rows, 2, 64, 0.2, out=torch.zeros_like(q[:n]))
+        pool.check_status()
+        got = pool.decode(0, q[:n], p.query_start_loc, p.ctx_lens, p.rows, 1, 64, 0.2, out=torch.zeros_like(q[:n]))
+        torch.cuda.synchronize()
+        code = int(pool.status.item())
+        pool.status.zero_()
+        if good or D == 48:
+            assert code == 0 and torch.equal(got, want), rows
+        else:
+            assert code == _lib.DEV_BAD_PLAN, rows
+
+
+def test_the_largest_plan():
+    """8192 items over 262144 rows and a cluster of the most CTAs."""
+    import cloverinfer_b200 as cb
+    i32 = dict(dtype=torch.int32, device="cuda")
+    n, rows, m = 8192, 1 << 18, 8192 * 9
+    g = torch.Generator().manual_seed(2)
+    at = torch.randperm(rows, generator=g)[:n].int().cuda()
+    new = torch.randint(0, 10, (n,), generator=g).int().cuda()
+    top, qsl = torch.tensor([n], **i32), torch.zeros(n + 1, **i32)
+    ctx, slots = torch.zeros(m, **i32), torch.zeros(m, dtype=torch.int64, device="cuda")
+    tables, tl, sl, st = torch.full((rows, 1), -1, **i32), torch.zeros(rows, **i32), torch.zeros(rows, **i32), torch.zeros(1, **i32)
+    cb.plan_step(torch.arange(n, **i32), top, tables, tl, sl, at, new, 16, qsl, ctx, slots, st)
+    assert int(st.item()) == 0
+    off = torch.nn.functional.pad(new.cumsum(0), (1, 0)).int()
+    assert torch.equal(qsl, off) and torch.equal(sl[at.long()], new)
+    used = new > 0
+    assert torch.equal(tables[at.long(), 0][used], n - used.int().cumsum(0)[used].int())
+    item = torch.repeat_interleave(torch.arange(n, device="cuda"), new.long())
+    total = item.numel()
+    pos = torch.arange(total, device="cuda") - off[item]
+    assert torch.equal(ctx[:total].long(), pos + 1) and bool((ctx[total:] == 0).all())
+    assert torch.equal(slots[:total], tables[at.long(), 0][item].long() * 16 + pos)
+    assert bool((slots[total:] == -1).all())
