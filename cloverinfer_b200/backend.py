@@ -704,7 +704,7 @@ class B200AttentionBackend:
             self._await_ingest()
         B = len(rows)
         meta = to_device_i32(rows + held + n_new, self.device)
-        pool.set_seq_lens(meta[:B], meta[B:2 * B])
+        pool.seq_lens.index_copy_(0, meta[:B].long(), meta[B:2 * B])
         p = pool.plan_step(meta[:B], meta[2 * B:], sum(n_new))
         for r, t, n in zip(rows, targets, n_new):
             if n:

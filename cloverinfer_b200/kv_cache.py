@@ -138,8 +138,10 @@ class PagedKVPool:
         self.free_top = torch.tensor([self.num_blocks], dtype=torch.int32, device=dev)
         self.tables = torch.full((self.max_seqs, self.max_blocks_per_seq), -1, dtype=torch.int32, device=dev)
         self.table_len = torch.zeros(self.max_seqs, dtype=torch.int32, device=dev)
-        # tokens held per row, for plan_step (the host paths do not use it)
-        self.seq_lens = torch.zeros(self.max_seqs, dtype=torch.int32, device=dev)
+        # tokens held per row, for plan_step (the host paths do not use it), and a
+        # place for those of rows outside the pool
+        self._seq_lens = torch.zeros(self.max_seqs + 1, dtype=torch.int32, device=dev)
+        self.seq_lens = self._seq_lens[:self.max_seqs]
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         # host mirror: counters only
         self.free_count = self.num_blocks
@@ -226,8 +228,10 @@ class PagedKVPool:
     # ------------------------------------------------------------ plan on the GPU
     def set_seq_lens(self, rows: torch.Tensor, lens: torch.Tensor) -> None:
         """Tell ``plan_step`` how many tokens rows hold (device int32 tensors): once per
-        sequence, and again when its row goes to another one."""
-        self.seq_lens.index_copy_(0, rows.long(), lens)
+        sequence, and again when its row goes to another one.  Rows outside the pool
+        (a plan's padding) are skipped."""
+        at = torch.where((rows >= 0) & (rows < self.max_seqs), rows, self.max_seqs)
+        self._seq_lens.index_copy_(0, at.long(), lens)
 
     def plan_step(self, rows: torch.Tensor, n_new: torch.Tensor, max_tokens: int) -> StepPlan:
         """Plan one step from ``seq_lens`` on the GPU: grow the tables of ``rows`` (device

@@ -49,3 +49,17 @@ def test_a_planned_step_refuses_requests_that_left():
         with pytest.raises(KeyError):
             be.decode_planned(step, 1, x, kv, kv)
         assert {r: q.layer_len for r, q in be._reqs.items()} == held
+
+
+def test_lengths_of_padding_rows_are_skipped():
+    """The rows of a plan may hold padding; out of the pool they index nothing."""
+    from cloverinfer_b200 import PagedKVPool
+    pool = PagedKVPool.__new__(PagedKVPool)
+    pool.max_seqs, pool._seq_lens = 4, torch.zeros(5, dtype=torch.int32)
+    pool.seq_lens = pool._seq_lens[:4]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    pool.set_seq_lens(i32([2, -1, 0, 9, -7]), i32([5, 6, 7, 8, 9]))
+    assert pool.seq_lens.tolist() == [7, 0, 5, 0]
+    pool.set_seq_lens(i32([]), i32([]))
+    pool.set_seq_lens(i32([3]), i32([1]))
+    assert pool.seq_lens.tolist() == [7, 0, 5, 1]
