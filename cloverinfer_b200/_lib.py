@@ -505,6 +505,10 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
             raise ValueError(f"{what}: norm_weight must be {d} contiguous float32 values")
     if rows == 0 or n_seqs == 0:
         return
+    # no context reaches past its table row (longer ones are flagged); the stride
+    # of a single row says nothing
+    width = block_tables.shape[1]
+    max_ctx_len = min(max_ctx_len, width * bs)
     if workspace is None:
         key = (dev, n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d, bs, k_cache.dtype,
                q.dtype, diff)
@@ -523,9 +527,9 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
             dtype_code(k_cache.dtype), nb, bs, _ptr(k_new), _ptr(v_new),
             0 if k_new is None else hkv * d if one else k_new.stride(0),
             0 if k_new is None else dtype_code(k_new.dtype),
-            block_tables.data_ptr(), block_tables.stride(0), _ptr(seq_rows), query_start_loc.data_ptr(),
-            ctx_lens.data_ptr(), n_seqs, rows, max_queries_per_seq, max_ctx_len, hq, hkv, d,
-            float(score_scale))
+            block_tables.data_ptr(), block_tables.stride(0) if block_tables.shape[0] > 1 else width,
+            _ptr(seq_rows), query_start_loc.data_ptr(), ctx_lens.data_ptr(), n_seqs, rows, max_queries_per_seq,
+            max_ctx_len, hq, hkv, d, float(score_scale))
     tail = (_ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
             _ptr(status))
     if diff:
@@ -544,6 +548,8 @@ def scaled_decode(out, q, k_cache, v_cache, k_scales, v_scales, block_tables, qu
     [num_blocks, bs, Hkv, D] int8 or float8_e4m3fn, scales [num_blocks, Hkv, bs]
     float32.  With k_new/v_new [rows, Hkv, D] every row's token is quantised into
     position ctx - 1 first.  Rows past ``query_start_loc[-1]`` are left as they were.
+    Contexts past ``max_ctx_len``, or past the columns of ``block_tables``, are cut off
+    there and set ``status``.
     ``workspace`` (attend_workspace_bytes) is allocated here by default."""
     _attend("scaled_decode", lib().clover_b200_scaled_decode, out, q, k_cache, v_cache, k_scales, v_scales,
             block_tables, query_start_loc, ctx_lens, max_queries_per_seq, max_ctx_len, score_scale, k_new,

@@ -419,6 +419,10 @@ __global__ void __launch_bounds__(256) attend_append_kernel(const AppendRowsArgs
     }
     const int pos = __ldg(a.ctx + r) - 1;
     if (pos < 0) continue;
+    if (pos >= a.max_ctx) {  // past what the attention covers
+      if (lane == 0) raise_status(a.status, CLOVER_B200_DEV_CTX_RANGE);
+      continue;
+    }
     const int trow = a.seq_rows ? __ldg(a.seq_rows + lo) : lo;
     const int bi = pos / a.bs, off = pos - bi * a.bs;
     const int blk = bi < a.table_stride ? __ldg(a.tables + (int64_t)trow * a.table_stride + bi) : -1;

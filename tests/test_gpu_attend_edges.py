@@ -162,3 +162,33 @@ def test_zero_and_tiny_value_rows(kv, q_dt):
         c.check(c.run(), f"V of 2^{e}")
         c.vs[c.tables[0, 7]] *= 2.0 ** 60  # a block of a far larger size among them
         c.check(c.run(), f"V of 2^{e} beside larger")
+
+
+# ---------------------------------------------------------------- contexts past the tables
+@pytest.mark.parametrize("kv,maps,D,new", [(I8, 1, 128, 1), (I8, 1, 128, 40), (F8, 1, 40, 1), (F16, 2, 128, 1), (F32, 2, 64, 1)])
+def test_contexts_past_the_table_columns(kv, maps, D, new):
+    """A view of some columns of wider tables: a longer context is cut off and
+    flagged, its new token written nowhere, and the other request is answered."""
+    from cloverinfer_b200 import _lib
+    for blocks in (3, 60):
+        n = 16 * blocks
+        c = Case([n + 5, n - 3], [1, min(new, n // 2)], hq=4, hkv=2, D=D, kv=kv, q_dt=F32 if kv != F16 else F16, maps=maps,
+                 seed=71)
+        kc, vc, ks, vs = c.append_reference()
+        page = int(c.tables[0, blocks])
+        for want, have in ((kc, c.kc), (vc, c.vc)) + (((ks.transpose(1, 2), c.ks.transpose(1, 2)),
+                                                       (vs.transpose(1, 2), c.vs.transpose(1, 2))) if ks is not None else ()):
+            want[page, 4] = have[page, 4]
+        wide = torch.full((2, blocks + 9), -1, dtype=torch.int32, device="cuda")
+        wide[:, 7:7 + blocks + 1] = c.tables[:, :blocks + 1]
+        full, c.tables = c.tables, wide[:, 7:7 + blocks]
+        out = c.run(step=True)
+        torch.cuda.synchronize()
+        assert int(c.status.item()) == _lib.DEV_CTX_RANGE
+        assert same_bytes(c.kc, kc) and same_bytes(c.vc, vc)
+        if ks is not None:
+            assert torch.equal(c.ks, ks) and torch.equal(c.vs, vs)
+        # the second request alone, over the full tables
+        c.tables, c.status = full, torch.zeros_like(c.status)
+        ref, tol = c.reference()
+        assert bool(((out.double() - ref).abs() <= tol)[1:c.T].all())

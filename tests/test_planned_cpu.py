@@ -63,3 +63,29 @@ def test_lengths_of_padding_rows_are_skipped():
     pool.set_seq_lens(i32([]), i32([]))
     pool.set_seq_lens(i32([3]), i32([1]))
     assert pool.seq_lens.tolist() == [7, 0, 5, 1]
+
+
+def _attend_args(monkeypatch, tables, max_ctx, rows=1, **kw):
+    """What a scaled_decode of host tensors would hand to the library."""
+    from cloverinfer_b200 import _lib
+    seen = {}
+    monkeypatch.setattr(_lib, "_one_device", lambda what, *ts: 0)
+    monkeypatch.setattr(_lib, "_call_on", lambda dev, fn, *args: seen.update(args=args) or 0)
+    c8, sc = torch.zeros(8, 16, 2, 64, dtype=torch.int8), torch.zeros(8, 2, 16)
+    x = torch.zeros(rows, 4, 64)
+    _lib.scaled_decode(x, x, c8, c8, sc, sc, tables, torch.arange(rows + 1, dtype=torch.int32),
+                       torch.ones(rows, dtype=torch.int32), max_queries_per_seq=1, max_ctx_len=max_ctx,
+                       score_scale=1.0, workspace=torch.zeros(1, dtype=torch.uint8), **kw)
+    return seen["args"][17], seen["args"][24]  # table stride, longest context
+
+
+def test_block_tables_of_one_row_and_of_some_columns(monkeypatch):
+    t = torch.zeros(3, 8, dtype=torch.int32)
+    assert _attend_args(monkeypatch, t, 100, 3) == (8, 100)
+    # one row: its stride says nothing (here 1 and 0)
+    col = torch.zeros(8, 1, dtype=torch.int32).t()
+    assert col.stride() == (1, 1) and _attend_args(monkeypatch, col, 100) == (8, 100)
+    assert _attend_args(monkeypatch, t[0].expand(1, 8), 128) == (8, 128)
+    # some columns: no context reaches past them into the next row's, or past the last row's end
+    assert _attend_args(monkeypatch, t[:, 6:], 100, 3) == (8, 32)
+    assert _attend_args(monkeypatch, t[1:2, 2:5], 100) == (3, 48)
