@@ -217,7 +217,7 @@ attend_generic_kernel(const AttendArgs a) {
             o[e] = lim[c] > 0 ? diff_value(o[e], acc[c2][e] * inv2, lam) : 0.f;
             sq = fmaf(o[e], o[e], sq);
           }
-          if (a.norm_w != nullptr) {
+          if (a.norm_w != nullptr && lim[c] > 0) {
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
             const float r = rsqrtf(sq / a.D + a.eps) * a.out_scale;
@@ -360,7 +360,7 @@ attend_join_kernel(const AttendArgs a, int wpo) {
       o[0][e] = diff_value(o[0][e], o[MAPS - 1][e], lam);
       sq = fmaf(o[0][e], o[0][e], sq);
     }
-    if (a.norm_w != nullptr) {
+    if (a.norm_w != nullptr && any) {
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
       const float r = rsqrtf(sq / a.D + a.eps) * a.out_scale;

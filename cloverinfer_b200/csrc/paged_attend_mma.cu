@@ -603,7 +603,7 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
         for (int h = 0; h < 2; ++h) {
           const int d = i * 16 + d0 + h * dh;
           const float w = a.norm_w != nullptr ? a.norm_w[d] : 1.f;
-          attend_store(a, ob + d, c.acc[i][2 * h] * (r * w));
+          attend_store(a, ob + d, any ? c.acc[i][2 * h] * (r * w) : 0.f);  // (0 * inf with eps = 0)
         }
       }
     }

@@ -192,3 +192,22 @@ def test_contexts_past_the_table_columns(kv, maps, D, new):
         c.tables, c.status = full, torch.zeros_like(c.status)
         ref, tol = c.reference()
         assert bool(((out.double() - ref).abs() <= tol)[1:c.T].all())
+
+
+# ---------------------------------------------------------------- rows without tokens under a norm
+@pytest.mark.parametrize("kv,D", [(F32, 64), (BF16, 128), (F16, 64), (I8, 128), (I8, 40)])
+@pytest.mark.parametrize("longest", [40, 900])
+def test_rows_without_tokens_are_zero_under_any_norm(kv, D, longest):
+    """Alone, and as the first row of several; eps = 0 makes their norm 0 / 0."""
+    import cloverinfer_b200 as cb
+    c = Case([0, 3, longest], [1, 4, 1], hq=4, hkv=2, D=D, kv=kv, q_dt=F32, maps=2, seed=81)
+    assert c.ctx_list == [0, 0, 1, 2, 3, longest]
+    for eps in (0.0, 1e-5):
+        out = torch.full_like(c.q, float("nan"))
+        cb.diff_decode(out, c.q, c.kc, c.vc, c.lam, c.tables, c.qsl, c.ctx, max_queries_per_seq=c.max_q,
+                       max_ctx_len=c.max_ctx, score_scale=c.scale, norm_weight=c.w, eps=eps, out_scale=0.6,
+                       k_scales=c.ks, v_scales=c.vs, status=c.status)
+        torch.cuda.synchronize()
+        assert bool((out[:2] == 0).all()), eps
+        assert bool(torch.isfinite(out).all())
+    c.check(out, "eps 1e-5")
