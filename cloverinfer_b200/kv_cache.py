@@ -84,13 +84,14 @@ class DiffAttention:
         return cls(lam.float().expand(num_heads).contiguous(), norm_weight, eps, 1.0 - float(lambda_init))
 
     def heads(self, lo: int, hi: int, device) -> "DiffAttention":
-        """The query heads [lo, hi) on ``device`` (this object if that is all of them, there)."""
-        device = torch.device(device)
-        if (lo, hi) == (0, self.lam.numel()) and self.lam.device == device:
+        """The query heads [lo, hi) as the decode takes them: on ``device``, float32 and
+        contiguous (this object if it is all of that already)."""
+        ready = lambda x: x.to(device=torch.device(device), dtype=torch.float32).contiguous()  # noqa: E731
+        lam = ready(self.lam if (lo, hi) == (0, self.lam.numel()) else self.lam[lo:hi])
+        w = None if self.norm_weight is None else ready(self.norm_weight)
+        if lam is self.lam and w is self.norm_weight:
             return self
-        w = None if self.norm_weight is None else self.norm_weight.to(device=device, dtype=torch.float32).contiguous()
-        return DiffAttention(self.lam[lo:hi].to(device=device, dtype=torch.float32).contiguous(), w, self.eps,
-                             self.out_scale)
+        return DiffAttention(lam, w, self.eps, self.out_scale)
 
 
 @dataclass
