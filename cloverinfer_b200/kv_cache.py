@@ -79,7 +79,11 @@ class DiffAttention:
                      eps: float = 1e-5) -> "DiffAttention":
         """From the learned vectors ([d], or [num_heads, d]): lam = exp(q1 . k1) -
         exp(q2 . k2) + lambda_init, computed once in 64 bits; the norm's output is
-        scaled by 1 - lambda_init."""
+        scaled by 1 - lambda_init.  ``norm_weight`` is needed (ones for a norm without
+        weights): only a norm's output takes that factor."""
+        if norm_weight is None:
+            raise ValueError("from_vectors: norm_weight is needed (ones for a norm without weights); for the bare "
+                             "difference of the maps construct DiffAttention(lam)")
         lam = (q1.double() * k1.double()).sum(-1).exp() - (q2.double() * k2.double()).sum(-1).exp() + lambda_init
         return cls(lam.float().expand(num_heads).contiguous(), norm_weight, eps, 1.0 - float(lambda_init))
 

@@ -28,6 +28,19 @@ def test_heads_makes_what_the_kernel_takes():
     assert fits.heads(0, 8, "cpu") is fits
 
 
+def test_from_vectors():
+    g = torch.Generator().manual_seed(0)
+    q1, k1, q2, k2 = (torch.randn(4, 32, generator=g) * 0.1 for _ in range(4))
+    w = torch.rand(64, generator=g)
+    d = DiffAttention.from_vectors(q1, k1, q2, k2, 0.2, 4, w)
+    want = torch.exp((q1.double() * k1.double()).sum(1)) - torch.exp((q2.double() * k2.double()).sum(1)) + 0.2
+    assert (d.lam.double() - want).abs().max() <= want.abs().max() * 2.0 ** -24
+    assert d.out_scale == 1 - 0.2 and d.norm_weight is w
+    # without a norm the output has no place for 1 - lambda_init
+    with pytest.raises(ValueError):
+        DiffAttention.from_vectors(q1, k1, q2, k2, 0.2, 4)
+
+
 @pytest.mark.parametrize("world", [1, 2, 3, 4, 8])
 def test_every_rank_has_the_lambdas_of_its_heads(world):
     """The shards' query heads, rank by rank, are all heads in order."""
