@@ -302,7 +302,7 @@ class B200AttentionBackend:
         ing = self._ingest_stream
         ing.wait_stream(cur)  # the blocks were reserved (and inputs made) on the decode stream
         on_host = not initial_kv[0]["key"].is_cuda
-        dtype = pool.new_dtype(initial_kv[0]["key"].dtype)
+        dtype = pool.new_dtype(*(layer[name].dtype for layer in initial_kv for name in ("key", "value")))
         with torch.cuda.stream(ing):
             shape = (L, 2, T, hl, self.head_dim)
             if on_host:
@@ -827,8 +827,8 @@ class B200AttentionBackend:
         sharded = self.shard is not None and self.shard.world > 1
         peer = self._peer_for(q) if sharded else None
         if self._own_attend:
-            if k_loc.dtype != v_loc.dtype:
-                k_loc, v_loc = k_loc.float(), v_loc.float()
+            dt = pool.new_dtype(k_loc.dtype, v_loc.dtype)
+            k_loc, v_loc = k_loc.to(dt), v_loc.to(dt)
             direct = dst is not None and not sharded and dst.dtype == q.dtype
             out = pool.attend(layer_idx, q, offs_d, ctx_d, rows_d, max(n_new), max(targets), score_scale,
                               k_new=k_loc, v_new=v_loc, diff=self._diff_layer(layer_idx, hq),

@@ -261,12 +261,12 @@ class PagedKVPool:
         self.row_blocks = self.table_len.tolist()
 
     # ------------------------------------------------------------ data path
-    def new_dtype(self, dtype: torch.dtype) -> torch.dtype:
-        """The dtype new K/V of ``dtype`` are handed to the append in: the cache's, or
-        for a scaled cache any float type as it is."""
+    def new_dtype(self, *dtypes: torch.dtype) -> torch.dtype:
+        """The dtype new K/V of these dtypes are handed to one append in: the cache's, or
+        for a scaled cache their own float type (float32 where they differ)."""
         if not self.scaled:
             return self.dtype
-        return dtype if dtype in _FLOATS else torch.float32
+        return dtypes[0] if len(set(dtypes)) == 1 and dtypes[0] in _FLOATS else torch.float32
 
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, slots: torch.Tensor) -> None:
         if self.scaled:
@@ -460,7 +460,7 @@ class KVCacheManager:
             pd = to_device_i32([0], dev)
             od = to_device_i32([0, n], dev)
             slots = self.pool.slots(rd, pd, od, n)
-            dt = self.pool.new_dtype(k_data.dtype)
+            dt = self.pool.new_dtype(k_data.dtype, v_data.dtype)
             k = k_data.to(device=dev, dtype=dt).contiguous()
             v = v_data.to(device=dev, dtype=dt).contiguous()
             self.pool.append(0, k, v, slots)
@@ -488,7 +488,7 @@ class KVCacheManager:
         row = self._rows[request_id]
         slots = self.pool.slots(to_device_i32([row], dev), to_device_i32([pos], dev),
                                 to_device_i32([0, 1], dev), 1)
-        dt = self.pool.new_dtype(k.dtype)
+        dt = self.pool.new_dtype(k.dtype, v.dtype)
         self.pool.append(0, k.to(device=dev, dtype=dt).reshape(1, self.num_heads, self.head_dim).contiguous(),
                          v.to(device=dev, dtype=dt).reshape(1, self.num_heads, self.head_dim).contiguous(),
                          slots)
