@@ -427,12 +427,12 @@ def kv_append_scaled(k_cache, v_cache, k_scales, v_scales, k_new, v_new, slot_ma
         raise TypeError(f"{what}: new K/V must be float32, float16 or bfloat16")
     if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or slot_mapping.numel() != n:
         raise ValueError(f"{what}: slot_mapping must be {n} contiguous int64 values")
-    if n == 0:
+    if n == 0 or layers == 0:
         return
     k0, v0 = (x.select(-3, 0) for x in (k_new, v_new))
     k0, v0 = (x[0] if many else x for x in (k0, v0))
     if (not (k0.is_contiguous() and v0.is_contiguous()) or (n > 1 and v_new.stride(-3) != k_new.stride(-3))
-            or (many and v_new.stride(0) != k_new.stride(0))):
+            or (layers > 1 and v_new.stride(0) != k_new.stride(0))):
         raise ValueError(f"{what}: each token's [H, D] row must be contiguous")
     rc = _call_on(dev, lib().clover_b200_kv_append_scaled, k_cache.data_ptr(), v_cache.data_ptr(),
                   k_scales.data_ptr(), v_scales.data_ptr(), _DTYPE[k_cache.dtype],

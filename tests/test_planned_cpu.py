@@ -89,3 +89,22 @@ def test_block_tables_of_one_row_and_of_some_columns(monkeypatch):
     # some columns: no context reaches past them into the next row's, or past the last row's end
     assert _attend_args(monkeypatch, t[:, 6:], 100, 3) == (8, 32)
     assert _attend_args(monkeypatch, t[1:2, 2:5], 100) == (3, 48)
+
+
+def test_one_layer_of_any_layer_stride(monkeypatch):
+    """The axis of a single layer: its stride says nothing."""
+    from cloverinfer_b200 import _lib
+    seen = {}
+    monkeypatch.setattr(_lib, "_one_device", lambda what, *ts: 0)
+    monkeypatch.setattr(_lib, "_call_on", lambda dev, fn, *args: seen.update(args=args) or 0)
+    c8, sc = torch.zeros(1, 4, 16, 2, 64, dtype=torch.int8), torch.zeros(1, 4, 2, 16)
+    x = torch.zeros(3, 2, 64)
+    _lib.kv_append_scaled(c8, c8, sc, sc, x[None], x.as_strided((1, 3, 2, 64), (7, 128, 64, 1)),
+                          torch.arange(3), None)
+    assert seen["args"][13:15] == (3, 1)  # tokens, layers
+    none = c8[:0], c8[:0], sc[:0], sc[:0], x[None][:0], x[None][:0]
+    assert _lib.kv_append_scaled(*none, torch.arange(3), None) is None
+    two = torch.zeros(2, 3, 2, 64)
+    with pytest.raises(ValueError):
+        _lib.kv_append_scaled(c8.repeat(2, 1, 1, 1, 1), c8.repeat(2, 1, 1, 1, 1), sc.repeat(2, 1, 1, 1),
+                              sc.repeat(2, 1, 1, 1), two, torch.zeros(4, 3, 2, 64)[::2], torch.arange(3), None)
