@@ -24,14 +24,12 @@ struct AppendScaledArgs {
 };
 
 // Rows of a multiple of 16 bytes, 16-byte aligned (dst: 8): a power of two of
-// lanes holds a row, up to 4 vectors each, and a thread has kAppendFlight rows
-// in flight; blockIdx.y is the layer, blockIdx.z K or V.  Bound: HBM (read the
-// row, write one byte per value), with the instructions close behind: one vector
-// per lane repeats the row's scale, slot and division in every lane (16381
-// tokens x 8 heads x 128, f16 -> e4m3: 46 us; a warp per row without vectors 92;
-// this 21.5, 72 % of the copy peak).
-constexpr int kAppendFlight = 1;  // (2: 27.5 us, fewer warps on an SM)
-
+// lanes holds a row, up to NV vectors each; blockIdx.y is the layer, blockIdx.z
+// K or V.  Bound: HBM (read the row, write one byte per value), with the
+// instructions close behind: one vector per lane repeats the row's scale, slot
+// and division in every lane (16381 tokens x 8 heads x 128, f16 -> e4m3: 46 us; a
+// warp per row without vectors 92; two rows in flight per thread, with fewer
+// warps on an SM, 27.5; this 21.5, 72 % of the copy peak).
 template <bool FP8, typename TI, int NV>
 __global__ void __launch_bounds__(256)
 kv_append_scaled_vec_kernel(const AppendScaledArgs a, int lpr) {
@@ -46,70 +44,60 @@ kv_append_scaled_vec_kernel(const AppendScaledArgs a, int lpr) {
   uint8_t* cache = (is_v ? a.vc : a.kc) + layer * a.cache_layer;
   float* scales = (is_v ? a.vs : a.ks) + layer * a.scale_layer;
   const int64_t step = (int64_t)gridDim.x * 8 * rpw;
-  for (int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * rpw + sub; r0 - sub < rows;
-       r0 += step * kAppendFlight) {
-    uint4 x[kAppendFlight][NV];
-    int64_t slot[kAppendFlight];
-    int head[kAppendFlight];
+  for (int64_t r = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * rpw + sub; r - sub < rows; r += step) {
+    uint4 x[NV];
+    int64_t slot = -1;
+    int head = 0;
 #pragma unroll
-    for (int f = 0; f < kAppendFlight; ++f) {
-      const int64_t r = r0 + f * step;
-      slot[f] = -1;
-      head[f] = 0;
+    for (int k = 0; k < NV; ++k) x[k] = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const int64_t t = rows <= INT32_MAX ? (int)r / a.heads : r / a.heads;
+      head = (int)(r - t * a.heads);
+      slot = __ldg(a.slots + t);
+      const uint4* row = reinterpret_cast<const uint4*>(src + t * a.new_token + (int64_t)head * a.dim);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) x[f][k] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int64_t t = rows <= INT32_MAX ? (int)r / a.heads : r / a.heads;
-        head[f] = (int)(r - t * a.heads);
-        slot[f] = __ldg(a.slots + t);
-        const uint4* row = reinterpret_cast<const uint4*>(src + t * a.new_token + (int64_t)head[f] * a.dim);
+      for (int k = 0; k < NV; ++k)
+        if (l + k * lpr < vecs) x[k] = __ldg(row + l + k * lpr);
+      if (slot >= a.n_slots) {
+        if (l == 0 && head == 0 && !is_v) raise_status(a.status, CLOVER_B200_DEV_BAD_SLOT);
+        slot = -1;
+      }
+    }
+    float v[NV][VEC];
+    uint32_t m = 0;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-          if (l + k * lpr < vecs) x[f][k] = __ldg(row + l + k * lpr);
-        if (slot[f] >= a.n_slots) {
-          if (l == 0 && head[f] == 0 && !is_v) raise_status(a.status, CLOVER_B200_DEV_BAD_SLOT);
-          slot[f] = -1;
+    for (int k = 0; k < NV; ++k) {
+      const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (VEC == 4) {
+          v[k][i] = __uint_as_float(w[i]);
+          m = max(m, abs_bits(v[k][i]));
+        } else {
+          const float2 p = Pack<TI>::unpack(w[i]);
+          v[k][2 * i] = p.x;
+          v[k][2 * i + 1] = p.y;
+          m = max(m, max(abs_bits(p.x), abs_bits(p.y)));
         }
       }
     }
+    for (int off = lpr >> 1; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+    float factor;
+    const float s = row_scale(m, code_top<FP8>(), factor);
+    if (slot < 0) continue;  // padding token
 #pragma unroll
-    for (int f = 0; f < kAppendFlight; ++f) {
-      float v[NV][VEC];
-      uint32_t m = 0;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const uint32_t w[4] = {x[f][k].x, x[f][k].y, x[f][k].z, x[f][k].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (VEC == 4) {
-            v[k][i] = __uint_as_float(w[i]);
-            m = max(m, abs_bits(v[k][i]));
-          } else {
-            const float2 p = Pack<TI>::unpack(w[i]);
-            v[k][2 * i] = p.x;
-            v[k][2 * i + 1] = p.y;
-            m = max(m, max(abs_bits(p.x), abs_bits(p.y)));
-          }
-        }
+    for (int k = 0; k < NV; ++k) {
+      if (l + k * lpr >= vecs) continue;
+      uint8_t* dst = cache + (slot * a.heads + head) * a.dim + (l + k * lpr) * VEC;
+      if constexpr (VEC == 4) {
+        *reinterpret_cast<uint32_t*>(dst) = encode4<FP8>(v[k], factor);
+      } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(encode4<FP8>(v[k], factor), encode4<FP8>(v[k] + 4, factor));
       }
-      for (int off = lpr >> 1; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
-      float factor;
-      const float s = row_scale(m, code_top<FP8>(), factor);
-      if (slot[f] < 0) continue;  // padding token
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        if (l + k * lpr >= vecs) continue;
-        uint8_t* dst = cache + (slot[f] * a.heads + head[f]) * a.dim + (l + k * lpr) * VEC;
-        if constexpr (VEC == 4) {
-          *reinterpret_cast<uint32_t*>(dst) = encode4<FP8>(v[k], factor);
-        } else {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(encode4<FP8>(v[k], factor), encode4<FP8>(v[k] + 4, factor));
-        }
-      }
-      if (l == 0) {
-        const int64_t blk = slot[f] <= INT32_MAX ? (int)slot[f] / a.bs : slot[f] / a.bs;
-        scales[(blk * a.heads + head[f]) * a.bs + (slot[f] - blk * a.bs)] = s;
-      }
+    }
+    if (l == 0) {
+      const int64_t blk = slot <= INT32_MAX ? (int)slot / a.bs : slot / a.bs;
+      scales[(blk * a.heads + head) * a.bs + (slot - blk * a.bs)] = s;
     }
   }
 }

@@ -18,8 +18,6 @@
 
 #include <mutex>
 
-#include <cudaTypedefs.h>
-
 namespace clover {
 
 template <typename KT>
@@ -208,8 +206,7 @@ attend_generic_kernel(const AttendArgs a) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) o[e] = lim[c] > 0 ? acc[c][e] * inv : 0.f;
         if (a.maps == 2) {
-          constexpr int kNext = 1;
-          const int c2 = c + kNext < NC ? c + kNext : c;
+          const int c2 = c + 1 < NC ? c + 1 : c;  // map 2 of the head (NC = 1 has one map)
           const float lam = a.lam[ci.head], inv2 = attend_inv(l[c2], lim[c2]);
           float sq = 0.f;
 #pragma unroll
