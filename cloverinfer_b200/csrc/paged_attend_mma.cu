@@ -39,20 +39,23 @@
 // and only one exponential is needed.  Weights are split into two 16-bit terms:
 // 2^-16 of the weight in bf16 (three terms, 2^-24, for fp32 queries); 2^-22 in
 // fp16 down to 2^-3, and half of fp16's least step, 2^-25, below.  fp16 weights
-// therefore stand high: a move of the reference puts the largest at 2^12, so
-// what is lost of a small one is at most 2^-37 of it.  (At 2^0, 40000 tokens
-// 18 nats below one with a V row of its own lost all that shared its piece, 9 to
-// 23 % of their sum; the sum of the weights itself is in fp32.)  fp32 queries are
-// split the same way (2^-22 of the column's largest over fp16 products, 2^-24
-// over bf16); columns of fp16 products are first scaled by a power of two so that
-// their largest value is in [2^14, 2^15).
+// are therefore multiplied by 2^12 before they are rounded (and the result by
+// 2^-12): what is lost of a small one is at most 2^-37 of the largest.  (Without
+// it 40000 tokens 18 nats below one with a V row of its own lost all that shared
+// its piece, 9 to 23 % of their sum.  The sum of the weights is in fp32.  The
+// factor is not part of the reference: 12 more in the exponential's argument
+// would round by 2^-21 of every weight.)  fp32 queries are split the same way
+// (2^-22 of a value over fp16 products, 2^-24 over bf16; a third fp16 term costs
+// 8 to 15 % and changes none of the errors measured); columns of fp16 products
+// are first scaled by a power of two so that their largest value is in
+// [2^14, 2^15).
 //
-// The reference moves only when a weight outgrows it: 2^15 for fp16 (2^3 above
-// the last move), 2^8 for bf16.  With the running maximum itself about half of
-// the stages of a worker rescaled the accumulators, and every stage took the
-// columns' maxima over the lanes; 2^8, 2^5 and 2^3 of room measure alike (64
-// ragged requests 124.0, 124.1, 124.1 us; scores five times as wide 124.4,
-// 124.6, 125.1).
+// The reference moves only when a weight exceeds it by 2^3 (fp16: 2^15 with the
+// factor) or 2^8 (bf16).  With the running maximum itself about half of the
+// stages of a worker rescaled the accumulators, and every stage took the columns'
+// maxima over the lanes; 2^8, 2^5 and 2^3 of room measure alike (64 ragged
+// requests 124.0, 124.1, 124.1 us; scores five times as wide 124.4, 124.6,
+// 125.1).
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -84,10 +87,10 @@ struct AttendGeom {
   static constexpr int kStageB = kTiles + kScales;
   static constexpr int kQTerms = !QF32 ? 1 : KV == KV_BF16 ? 3 : 2;
   static constexpr int kPTerms = KV == KV_BF16 && QF32 ? 3 : 2;
-  // Where a move of the reference puts the largest weight (log2), and the weight
-  // that makes it move.
-  static constexpr float kTopLog2 = KV == KV_BF16 ? 0.f : 12.f;
-  static constexpr float kMaxWeight = KV == KV_BF16 ? 256.f : 32768.f;
+  // What a weight is multiplied by before it is rounded, and the weight (before
+  // that) that makes the reference move.
+  static constexpr float kUp = KV == KV_BF16 ? 1.f : 4096.f;
+  static constexpr float kMaxWeight = KV == KV_BF16 ? 256.f : 8.f;
   // Warps: 16, 12 or 8 (128, 168 or 255 registers each), as many as hold
   // accumulators, query fragments and about 80 more, with rings at least two
   // stages deep.
@@ -181,7 +184,7 @@ constexpr float kNoRef = -1e30f;
 
 // V scales under 2^-80 count as that in the reference (a zero row's is 0, the
 // least stored 2^-109), though the weight takes them as they are: a softmax
-// weight is then at most 2^(15 + 80), and the sum of 2^31 of them finite.
+// weight is then at most 2^(3 + 80), and the sum of 2^31 of them finite.
 constexpr float kLeastScale = 8.271806125530277e-25f;
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -439,7 +442,8 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
     const int i = 2 * h + e;
     p[i] = masked(h, e) ? 0.f : fast_exp2(fmaf(s[i], c.sc[e], -c.m[e]));
     // (a masked token's scale may be anything: its weight stays 0)
-    w[i] = G::kEight ? (masked(h, e) ? 0.f : p[i] * vsc[h]) : p[i];
+    const float up = p[i] * G::kUp;
+    w[i] = G::kEight ? (masked(h, e) ? 0.f : up * vsc[h]) : up;
   };
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -457,7 +461,7 @@ __device__ __forceinline__ void attend_step(uint32_t ks, uint32_t vs, const uint
         if (!masked(h, e)) mx = fmaxf(mx, fmaf(s[2 * h + e], c.sc[e], G::kEight ? fast_log2(vref[h]) : 0.f));
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float nm = fmaxf(c.m[e], mx - G::kTopLog2);
+      const float nm = fmaxf(c.m[e], mx);
       const float al = fast_exp2(c.m[e] - nm);
       c.m[e] = nm;
       c.l[e] *= al;
@@ -537,6 +541,7 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
                                              AttendCols<KV, QF32, D, CW>& c, int lane) {
   using G = AttendGeom<KV, QF32, D, CW>;
   constexpr int KK = D / 16, COLS = 8 * CW;
+  constexpr float kDown = 1.f / G::kUp;  // (a power of two: exact)
   const bool whole = a.whole || (first_jj == 0 && cur.jj == cur.s.n - 1);
 #pragma unroll
   for (int off = 4; off < 32; off <<= 1) {
@@ -554,10 +559,10 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
 #pragma unroll
       for (int i = 0; i < KK; ++i) {
         if (G::kEight) {
-          *reinterpret_cast<float2*>(po + i * 16 + d0) = make_float2(c.acc[i][e], c.acc[i][2 + e]);
+          *reinterpret_cast<float2*>(po + i * 16 + d0) = make_float2(c.acc[i][e] * kDown, c.acc[i][2 + e] * kDown);
         } else {
-          po[i * 16 + d0] = c.acc[i][e];
-          po[i * 16 + d0 + dh] = c.acc[i][2 + e];
+          po[i * 16 + d0] = c.acc[i][e] * kDown;
+          po[i * 16 + d0 + dh] = c.acc[i][2 + e] * kDown;
         }
       }
       if (lane < 4) a.part_ml[at] = make_float2(c.m[e], c.l[e]);
@@ -568,7 +573,7 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
       const AttendCol ci = attend_col(a, cur.s.row0, cur.s.nq, kvh, chunk * COLS + c0 + e);
       if (!ci.valid) continue;
       const bool any = c.lim[e] > 0;
-      const float inv = attend_inv(c.l[e], c.lim[e]);
+      const float inv = attend_inv(c.l[e], c.lim[e]) * kDown;
       const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D + d0;
 #pragma unroll
       for (int i = 0; i < KK; ++i) {
@@ -581,7 +586,7 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
     const AttendCol ci = attend_col(a, cur.s.row0, cur.s.nq, kvh, chunk * COLS + c0);
     const bool any = c.lim[0] > 0;
     const float lam = ci.valid ? a.lam[ci.head] : 0.f;
-    const float i0 = attend_inv(c.l[0], c.lim[0]), i1 = attend_inv(c.l[1], c.lim[1]);
+    const float i0 = attend_inv(c.l[0], c.lim[0]) * kDown, i1 = attend_inv(c.l[1], c.lim[1]) * kDown;
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < KK; ++i) {
@@ -596,14 +601,15 @@ __device__ __forceinline__ void finish_piece(const AttendArgs& a, const Cursor& 
     for (int off = 4; off < 32; off <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
     if (ci.valid) {
       const int64_t ob = (int64_t)ci.row * a.out_stride + (int64_t)ci.head * D;
-      const float r = a.norm_w != nullptr ? rsqrtf(sq / D + a.eps) * a.out_scale : 1.f;
+      // (a row without tokens is 0, and eps may be)
+      const float r = a.norm_w == nullptr ? 1.f : any ? rsqrtf(sq / D + a.eps) * a.out_scale : 0.f;
 #pragma unroll
       for (int i = 0; i < KK; ++i) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int d = i * 16 + d0 + h * dh;
           const float w = a.norm_w != nullptr ? a.norm_w[d] : 1.f;
-          attend_store(a, ob + d, any ? c.acc[i][2 * h] * (r * w) : 0.f);  // (0 * inf with eps = 0)
+          attend_store(a, ob + d, c.acc[i][2 * h] * (r * w));
         }
       }
     }

@@ -140,8 +140,8 @@ def test_many_small_weights_beside_a_large_one(kv, maps, bits):
 @pytest.mark.parametrize("kv", [I8, F8])
 @pytest.mark.parametrize("q_dt", [F32, BF16])
 def test_zero_and_tiny_value_rows(kv, q_dt):
-    """Thousands of zero V rows with the largest scores before the others; V rows so
-    small that a weight times their scale is far below fp16."""
+    """Thousands of zero V rows before the others; V rows so small, or so large, that
+    a weight times their scale is far outside fp16."""
     c = Case([6000, 40, 3000], hq=8, hkv=2, kv=kv, q_dt=q_dt, seed=61, spread=False)
     ids = c.tables[0, :300].long()  # 4800 tokens
     c.vc.view(torch.uint8)[ids] = 0
@@ -156,12 +156,12 @@ def test_zero_and_tiny_value_rows(kv, q_dt):
     out = c.run()
     c.check(out, "nothing but zeros")
     assert bool((out[2] == 0).all())
-    for e in (-40, -84):
+    for e in (-40, -84, 115):
         c = Case([700, 40, 100], hq=8, hkv=2, kv=kv, q_dt=q_dt, seed=62, spread=False)
         c.vs *= 2.0 ** e
         c.check(c.run(), f"V of 2^{e}")
-        c.vs[c.tables[0, 7]] *= 2.0 ** 60  # a block of a far larger size among them
-        c.check(c.run(), f"V of 2^{e} beside larger")
+        c.vs[c.tables[0, 7]] *= 2.0 ** (60 if e < 0 else -60)  # a block of a far other size among them
+        c.check(c.run(), f"V of 2^{e} beside others")
 
 
 # ---------------------------------------------------------------- contexts past the tables
