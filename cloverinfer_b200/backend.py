@@ -36,7 +36,7 @@ step once for all layers on the GPU, and ``decode_planned`` runs a layer of it.
 the cache in 8 bits with a scale per token and KV head; ``differential`` gives
 each layer's differential attention (``DiffAttention``: two softmax maps over the
 halves of head_dim, their difference normed).  Both run on every path above;
-sharded, their outputs go through NCCL.
+sharded, their steps are not captured and the outputs go through NCCL.
 """
 
 from __future__ import annotations
@@ -675,9 +675,9 @@ class B200AttentionBackend:
 
     def begin_step(self, request_ids: Sequence[str], n_new: Optional[Sequence[int]] = None) -> PlannedStep:
         """Plan a step of ``n_new[b]`` new tokens per request (default 1) once for all
-        layers: one small copy of rows and lengths, and one launch that grows the block
-        tables and lays out slots, contexts and query offsets on the GPU
-        (``clover_b200_plan_step``).  Run it with ``decode_planned``, every layer once.
+        layers: one small copy of rows and lengths, two small kernels that set the lengths
+        held, and one launch that grows the block tables and lays out slots, contexts and
+        query offsets on the GPU (``clover_b200_plan_step``).  Run it with ``decode_planned``, every layer once.
         Raises before any state changes, like ``decode_batch``; a request's layers must
         hold the same number of tokens."""
         pool = self.pool

@@ -93,7 +93,7 @@ struct AttendGeom {
   static constexpr float kMaxWeight = KV == KV_BF16 ? 256.f : 8.f;
   // Warps: 16, 12 or 8 (128, 168 or 255 registers each), as many as hold
   // accumulators, query fragments and about 80 more, with rings at least two
-  // stages deep.
+  // stages deep; 6 where 8 such rings do not fit (head_dim 256 in 16 bits).
   static constexpr int kRegs = D / 4 + D / 8 * kQTerms + (kEight ? 92 : 80);
   static constexpr int kBudget = 232448 - 1024 - 1024;  // an SM's shared memory, less alignment and barriers
   static constexpr int kWarps = kRegs <= 128 && attend_fits(16 / CW, kStageB, kBudget)   ? 16

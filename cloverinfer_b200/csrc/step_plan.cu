@@ -10,7 +10,9 @@
 // popped block free_stack[top - 1 - (growth of the items before i + k - table_len[row])]:
 // the pops of clover_b200_block_reserve (KVCacheManager.allocate / append_slot,
 // src/core/memory_manager.py:55-72, :95-121) in the same order, so a token's
-// slot needs no wait for the table to be written.
+// slot needs no wait for the table to be written.  A block id outside the cache
+// (a damaged table or stack) raises BAD_BLOCK and gives its tokens slot -1; the
+// state is committed all the same.
 //
 // Bound: launch latency and three dependent loads (rows, lengths, block ids)
 // for a decode step; for admissions of whole prompts the 12 bytes written per

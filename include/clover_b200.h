@@ -418,7 +418,9 @@ CLOVER_B200_API int clover_b200_paged_decode_noalloc(void* out, int64_t out_row_
  * the tables have num_rows rows.  All or nothing: if the blocks, a table row
  * or max_tokens do not hold the step, or a row is out of range or stands in
  * the batch twice, the status word gets OOM, TABLE_FULL or BAD_PLAN, no state
- * changes and the layout is empty (zeros and -1).  At most 8192 items and
+ * changes and the layout is empty (zeros and -1).  (A damaged allocator state, a
+ * table entry or popped id outside the cache, is no such case: BAD_BLOCK, slot
+ * -1 for its tokens, and the rest of the step is made.)  At most 8192 items and
  * 262144 rows.  Calls on one allocator state must be ordered by the caller.
  * Replaces: append_slot for every request of a step (memory_manager.py:95-121)
  * with get_kernel_inputs (:145-173).
@@ -457,7 +459,8 @@ CLOVER_B200_API int clover_b200_kv_append_scaled(void* k_cache, void* v_cache, f
 /*
  * Bytes of workspace clover_b200_scaled_decode (differential = 0) or
  * clover_b200_diff_decode (1) needs for a call of these sizes; 0 for short
- * contexts, -1 on invalid sizes.  It does not grow with the batch.
+ * contexts, -1 on invalid sizes.  The partials do not grow with the batch;
+ * beside them it holds 16 bytes per (sequence, KV head, column chunk).
  */
 CLOVER_B200_API int64_t clover_b200_attend_workspace_bytes(int32_t n_seqs, int32_t n_query_rows,
                           int32_t max_queries_per_seq, int32_t max_ctx_len, int32_t num_q_heads,
@@ -470,7 +473,8 @@ CLOVER_B200_API int64_t clover_b200_attend_workspace_bytes(int32_t n_seqs, int32
  * v_scales * codes; queries and outputs f32, f16 or bf16.  k_new / v_new (may
  * be NULL; new_dtype f32, f16 or bf16): every query row's new token is
  * quantised into position ctx_lens[r] - 1 first, as in
- * clover_b200_decode_step.  Within a sequence ctx_lens must not decrease.  Rows
+ * clover_b200_decode_step; one whose block id is bad, or past max_ctx_len, is
+ * not written.  A row without tokens is zero.  Within a sequence ctx_lens must not decrease.  Rows
  * at and past query_start_loc[n_seqs] are not touched; a masked token adds
  * nothing, whatever it holds.  head_dim up to 256, any block_size; head_dim
  * 64/128/256 with a block_size that is a multiple of 16 takes the tensor-core
