@@ -527,7 +527,7 @@ def _attend(what, fn, out, q, k_cache, v_cache, k_scales, v_scales, block_tables
             dtype_code(k_cache.dtype), nb, bs, _ptr(k_new), _ptr(v_new),
             0 if k_new is None else hkv * d if one else k_new.stride(0),
             0 if k_new is None else dtype_code(k_new.dtype),
-            block_tables.data_ptr(), block_tables.stride(0) if block_tables.shape[0] > 1 else width,
+            block_tables.data_ptr(), block_tables.stride(0) if block_tables.shape[0] > 1 else max(width, 1),
             _ptr(seq_rows), query_start_loc.data_ptr(), ctx_lens.data_ptr(), n_seqs, rows, max_queries_per_seq,
             max_ctx_len, hq, hkv, d, float(score_scale))
     tail = (_ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),

@@ -86,6 +86,8 @@ def test_block_tables_of_one_row_and_of_some_columns(monkeypatch):
     col = torch.zeros(8, 1, dtype=torch.int32).t()
     assert col.stride() == (1, 1) and _attend_args(monkeypatch, col, 100) == (8, 100)
     assert _attend_args(monkeypatch, t[0].expand(1, 8), 128) == (8, 128)
+    # no columns (a batch without tokens)
+    assert _attend_args(monkeypatch, t[:1, :0], 0)[0] >= 1
     # some columns: no context reaches past them into the next row's, or past the last row's end
     assert _attend_args(monkeypatch, t[:, 6:], 100, 3) == (8, 32)
     assert _attend_args(monkeypatch, t[1:2, 2:5], 100) == (3, 48)
